@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define TRT_ABI_VERSION 9
+#define TRT_ABI_VERSION 10
 
 #define TRT_OK 0
 #define TRT_E_INVALID (-1)   /* null pointer, non-positive size, bad enum   */
@@ -299,6 +299,30 @@ size_t trt_mm_workspace_bytes(int64_t m, int64_t k, int64_t n, int variant, int 
  */
 int trt_mm_bf16(const float *a, const float *b, float *c, int64_t m, int64_t k, int64_t n,
                 int pieces, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Products of ragged groups ("experts"): T rows lie in E consecutive groups of sizes[e] rows, and
+ * every group has its own matrix.  sizes: E values on the device, int32, or int64 with wide_sizes != 0;
+ * the host never reads them.  Rows behind the last group belong to none; sizes that are negative or
+ * reach past T in sum are clamped (no sizes make a kernel leave the tensors).  dtype: TRT_BF16, TRT_F16 or
+ * TRT_F32; sums are fp32 (fp32 products in IEEE fp32 on the fp32 matrix pipe) and a result is rounded once.  No
+ * counterpart in the reference, whose mm has one matrix (triturus/mm.py:181-214).
+ *
+ * trt_gmm: c[r, n] = sum_k a[r, k] b[e(r), k, n]; a: T x K with row stride lda and unit trailing stride,
+ * b: E x K x N with element strides sb, of which sb[1] or sb[2] is 1 (TRT_E_LAYOUT otherwise; a transposed view is
+ * read in place), c: T x N, dense.  Rows of c behind the last group are set to zero.  With g for
+ * a and b's last two strides exchanged it makes a's gradient.
+ * trt_gmm_weights: d[e, k, n] = sum_{r in e} a[r, k] g[r, n], the gradient of b; d: E x K x N, dense; zeros
+ * for a group without rows.
+ * 16-byte loads of whole chunks where bases and strides allow (all of them multiples of 16 bytes), otherwise chunks
+ * from any address with the ends of rows read value by value.  A row may be at most 8 MiB long or apart
+ * (TRT_E_RANGE).  tile: 0 = choose by shape, 1..TRT_GMM_TILES force a tile (experiments, tests).
+ */
+#define TRT_GMM_TILES 2
+int trt_gmm(const void *a, const void *b, const void *sizes, void *c, int64_t T, int64_t E, int64_t K,
+            int64_t N, int64_t lda, const int64_t sb[3], int dtype, int wide_sizes, int tile, void *stream);
+int trt_gmm_weights(const void *a, const void *g, const void *sizes, void *d, int64_t T, int64_t E, int64_t K,
+                    int64_t N, int64_t lda, int64_t ldg, int dtype, int wide_sizes, int tile, void *stream);
 
 /*
  * r = x + y for contiguous vectors of n elements of `dtype` (TRT_F32 ...).  Replaces the

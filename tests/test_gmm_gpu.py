@@ -1,0 +1,213 @@
+"""gmm and gmm_grad against the definition in 64 bits.
+
+Tolerance of one value: operands are exact in 64 bits; products of 16-bit values are exact in fp32, fp32
+products and every addition round by at most 2^-23 of the running sum of magnitudes (truncation counted), so the
+sum is off by at most (terms + 1) 2^-23 sum |x||y|, and the result's own rounding by eps / 2 of its value (and half
+the smallest subnormal step of the type).
+"""
+
+import math
+
+import pytest
+import torch
+
+from triturus_amd.gmm import gmm, gmm_grad
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def product64(a, b, sizes):
+    c = torch.zeros(a.shape[0], b.shape[2], dtype=torch.float64, device=a.device)
+    r = 0
+    for e, n in enumerate(sizes):
+        c[r:r + n] = a[r:r + n].double() @ b[e].double()
+        r += n
+    return c
+
+
+def weights64(a, g, sizes):
+    d, r = [], 0
+    for n in sizes:
+        d.append(a[r:r + n].double().T @ g[r:r + n].double())
+        r += n
+    return torch.stack(d)
+
+
+def close(got, want, magnitude, terms):
+    info = torch.finfo(got.dtype)
+    bound = (info.eps / 2) * want.abs() + (terms + 1) * 2.0 ** -23 * magnitude + info.smallest_normal * info.eps / 2
+    bad = ~((got.double() - want).abs() <= bound * (1 + 2 ** -8))  # the rounding counts the rounded value's binade
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} values off, worst {float((got.double() - want).abs()[bad].max())}"
+
+
+def operands(dev, T, E, K, N, dtype, layout="kn"):
+    a = torch.randn(T, K, device=dev).to(dtype)
+    b = (torch.randn(E, K, N, device=dev) if layout == "kn" else torch.randn(E, N, K, device=dev)).to(dtype)
+    return a, (b if layout == "kn" else b.transpose(1, 2)), torch.randn(T, N, device=dev).to(dtype)
+
+
+def check(a, b, g, sizes, wide=False):
+    dev = a.device
+    s = torch.tensor(sizes, dtype=torch.int64 if wide else torch.int32, device=dev)
+    c = gmm(a, b, s)
+    assert c.shape == g.shape and c.dtype == a.dtype and c.is_contiguous()
+    close(c, product64(a, b, sizes), product64(a.abs(), b.abs(), sizes), a.shape[1])
+    da, db = gmm_grad(g, a, b, s)
+    assert da.shape == a.shape and db.shape == b.shape and da.dtype == db.dtype == a.dtype
+    bt = b.transpose(1, 2)
+    close(da, product64(g, bt, sizes), product64(g.abs(), bt.abs(), sizes), b.shape[2])
+    close(db, weights64(a, g, sizes), weights64(a.abs(), g.abs(), sizes), max([1] + sizes))
+    return c, da, db
+
+
+SHAPES = [  # sizes, K, N, rows behind the last group
+    ([1], 1, 1, 0), ([0], 5, 3, 1), ([1, 0, 1], 8, 8, 0), ([3, 0, 5, 1], 64, 128, 2), ([0, 0, 130], 72, 136, 0),
+    ([127, 128, 129, 1], 128, 128, 7), ([257], 200, 264, 0), ([33, 0, 64, 65, 31, 2], 129, 77, 11), ([300, 5], 65, 1, 3),
+    ([5, 300], 1, 65, 0), ([16] * 70, 96, 40, 5), ([1] * 130 + [0] * 10 + [40], 64, 64, 0), ([512, 0, 512], 256, 512, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_products_and_gradients(dev, shape, layout, dtype):
+    sizes, K, N, tail = SHAPES[shape]
+    check(*operands(dev, sum(sizes) + tail, len(sizes), K, N, dtype, layout), sizes, wide=shape % 2 == 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("T,E", [(2, 64), (40, 3), (130, 2), (700, 4), (2500, 5)])
+def test_sizes_over_the_tiles(dev, T, E, dtype):
+    cut = torch.sort(torch.randint(0, T + 1, (E - 1,)))[0].tolist()
+    sizes = [y - x for x, y in zip([0] + cut, cut + [T])]
+    for K, N in ((64, 256), (264, 520), (515, 300)):
+        check(*operands(dev, T, E, K, N, dtype), sizes)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_views_are_read_in_place(dev, dtype):
+    sizes, K, N = [20, 0, 50], 48, 72
+    a, b, g = operands(dev, 70, 3, K, N, dtype)
+    for off in (0, 1, 8):  # offsets and row lengths that leave and keep 16-byte boundaries
+        wide_a, wide_b, wide_g = (torch.full((*t.shape[:-1], t.shape[-1] + 16), math.nan, device=dev, dtype=dtype) for t in (a, b, g))
+        va, vb, vg = (w[..., off:off + t.shape[-1]].copy_(t) for w, t in ((wide_a, a), (wide_b, b), (wide_g, g)))
+        check(va, vb, vg, sizes)
+    check(a[:, ::2], b[:, ::2, ::3], g[:, ::3], sizes)  # no unit stride: copied
+    check(a[:1].expand(70, K), b[:1].expand(3, K, N), g[:1].expand(70, N), sizes)
+    s = torch.tensor([20, 9, 0, 9, 50], dtype=torch.int32, device=dev)[::2]
+    assert torch.equal(gmm(a, b, s), gmm(a, b, s.clone()))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_neighbours_do_not_leak(dev, dtype):
+    """NaN and infinity in other groups, in the rows behind the last group and in other matrices stay there."""
+    sizes, K, N = [37, 0, 21, 64], 40, 56
+    a, b, g = operands(dev, 130, 4, K, N, dtype)
+    clean = check(a, b, g, sizes)
+    a[37:58], g[37:58], b[1] = math.nan, math.inf, math.nan
+    a[122:], g[122:] = math.inf, math.nan
+    s = torch.tensor(sizes, device=dev)
+    c, (da, db) = gmm(a, b, s), gmm_grad(g, a, b, s)
+    keep = torch.ones(130, dtype=torch.bool, device=dev)
+    keep[37:58] = False
+    assert torch.equal(c[keep], clean[0][keep]) and torch.equal(da[keep], clean[1][keep])
+    assert c[37:58].isnan().all() and not c[122:].any() and not da[122:].any()
+    assert torch.equal(db[[0, 1, 3]], clean[2][[0, 1, 3]]) and db[2].isnan().all()
+
+
+@pytest.mark.parametrize("sizes", [[5, -3, 9, 4], [10, 100, 7, 3], [1 << 30, 1 << 30, 1 << 30, 1 << 30], [-1, -1, -1, -1]])
+def test_sizes_that_do_not_fit_are_clamped(dev, sizes):
+    T, K, N = 40, 24, 32
+    a, b, g = operands(dev, T, 4, K, N, torch.float32)
+    fit, left = [], T
+    for n in sizes:
+        fit.append(min(max(n, 0), left))
+        left -= fit[-1]
+    for dtype in (torch.int32, torch.int64):
+        s = torch.tensor(sizes, dtype=dtype, device=dev)
+        want = torch.tensor(fit, dtype=dtype, device=dev)
+        assert torch.equal(gmm(a, b, s), gmm(a, b, want))
+        for x, y in zip(gmm_grad(g, a, b, s), gmm_grad(g, a, b, want)):
+            assert torch.equal(x, y)
+
+
+def test_empty_operands(dev):
+    s = torch.tensor([0, 0], device=dev)
+    a, b = torch.empty(0, 8, device=dev), torch.randn(2, 8, 4, device=dev)
+    assert gmm(a, b, s).shape == (0, 4)
+    da, db = gmm_grad(torch.empty(0, 4, device=dev), a, b, s)
+    assert da.shape == (0, 8) and not db.any() and db.shape == b.shape
+    s = torch.tensor([3, 0], device=dev)
+    assert not gmm(torch.empty(5, 0, device=dev), torch.empty(2, 0, 4, device=dev), s).any()
+    assert gmm(torch.randn(5, 8, device=dev), torch.empty(2, 8, 0, device=dev), s).shape == (5, 0)
+    da, db = gmm_grad(torch.empty(5, 0, device=dev), torch.randn(5, 8, device=dev), torch.empty(2, 8, 0, device=dev), s)
+    assert da.shape == (5, 8) and not da.any() and db.shape == (2, 8, 0)
+
+
+def test_autograd_matches_differences(dev):
+    """The gradient of sum(g c) is linear in each operand: c(a + h) - c(a) along a direction, in 64 bits, is exact."""
+    sizes = torch.tensor([7, 0, 12], dtype=torch.int32, device=dev)
+    a, b, g = operands(dev, 21, 3, 10, 14, torch.float32)
+    a.requires_grad_(), b.requires_grad_()
+    (gmm(a, b, sizes) * g).sum().backward()
+    da, db = torch.randn_like(a), torch.randn_like(b)
+    value = lambda x, y: (product64(x, y, [7, 0, 12]) * g.double()).sum()  # noqa: E731
+    with torch.no_grad():
+        up = value(a.double() + da.double(), b) - value(a, b)
+        along = (a.grad.double() * da).sum()
+        scale = (product64(g.abs(), b.abs().transpose(1, 2), [7, 0, 12]) * da.abs()).sum()
+        assert abs(up - along) <= 16 * 2.0 ** -23 * scale
+        up = value(a, b.double() + db.double()) - value(a, b)
+        along = (b.grad.double() * db).sum()
+        scale = (weights64(a.abs(), g.abs(), [7, 0, 12]) * db.abs()).sum()
+        assert abs(up - along) <= 22 * 2.0 ** -23 * scale
+    # one operand alone, a product that is summed (an expanded gradient), a shared matrix
+    x = a.detach().clone().requires_grad_()
+    gmm(x, b.detach(), sizes).sum().backward()
+    assert torch.equal(x.grad, gmm_grad(torch.ones_like(g), x.detach(), b.detach(), sizes)[0])
+    w = b.detach()[:1].clone().requires_grad_()
+    (gmm(a.detach(), w.expand(3, -1, -1), sizes) * g).sum().backward()
+    each = gmm_grad(g, a.detach(), w.detach().expand(3, -1, -1), sizes)[1]
+    assert torch.equal(w.grad, each.sum(0, keepdim=True))
+
+
+def test_graph_and_streams(dev):
+    sizes = [100, 0, 60, 40]
+    a, b, g = operands(dev, 210, 4, 96, 136, torch.bfloat16)
+    s = torch.tensor(sizes, device=dev)
+    want = (gmm(a, b, s), *gmm_grad(g, a, b, s))
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = (gmm(a, b, s), *gmm_grad(g, a, b, s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want, other))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = (gmm(a, b, s), *gmm_grad(g, a, b, s))
+    for turn in ([50, 50, 50, 50], [0, 200, 10, 0], sizes):  # sizes change between replays
+        s.copy_(torch.tensor(turn))
+        eager = (gmm(a, b, s), *gmm_grad(g, a, b, s))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, eager))
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            gmm(a.clone().requires_grad_(), b, s)
+    torch.cuda.synchronize()
+    assert torch.equal(gmm(a, b, s), want[0])
+
+
+def test_refusals(dev):
+    a, b, g = operands(dev, 6, 2, 8, 4, torch.float32)
+    s = torch.tensor([3, 3], device=dev)
+    for bad in ((a[0], b, s), (a, b[0], s), (a, b, s[None]), (a[:, :7], b, s), (a, b, s[:1]), (a.half(), b, s), (a, b, s.float()),
+                (a, b, s.cpu()), (a, b[:0], s[:0])):
+        with pytest.raises(AssertionError):
+            gmm(*bad)
+    with pytest.raises(NotImplementedError):
+        gmm(a.double(), b.double(), s)
+    for bad in (g[:, :3], g.half(), g.cpu()):
+        with pytest.raises(AssertionError):
+            gmm_grad(bad, a, b, s)

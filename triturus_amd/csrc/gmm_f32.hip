@@ -1,0 +1,10 @@
+// The products of ragged groups for f32 operands (a file of its own per type: they compile side by side).
+#include "gmm_launch.hpp"
+
+namespace trt {
+
+int gmm_f32(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, hipStream_t s) {
+    return launch_gmm_type<float>(g, E, T_rows, weights, y_inner, tile, s);
+}
+
+}  // namespace trt

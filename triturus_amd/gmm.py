@@ -1,0 +1,145 @@
+"""gmm: matrix products grouped by expert, with ragged sizes, on MI355X.
+
+``mm`` (triturus/mm.py:181-214) has one matrix for all rows; here T rows lie in E consecutive groups of
+``sizes[e]`` rows and every group has its own matrix: the products of a mixture layer.  The reference has no
+counterpart.  ``sizes`` stays on the device (nothing here waits for it), so a router's output can be passed on.
+
+    c = gmm(a, b, sizes)                  # a: T x K, b: E x K x N, sizes: E  ->  c: T x N
+    da, db = gmm_grad(g, a, b, sizes)     # of sum(g * c)
+
+Types: bfloat16, float16 and float32, one for all operands.  Sums are fp32; a result is rounded once to the
+operands' type.  fp32 contracts in IEEE fp32 on the fp32 matrix pipe whatever ``set_tf32_enabled`` says.
+Rows behind the last group (a padded batch) give zeros, take no gradient and are never read as terms of a sum.
+Groups may be empty.  Sizes that are negative or reach past T in sum are clamped: nothing outside the tensors is touched.
+
+``gmm`` takes part in autograd.  Under HIP graph capture it refuses operands that require a gradient: capture
+``gmm`` on detached operands and ``gmm_grad`` instead (a backward pass of autograd captured while another graph
+of the same leaves is alive ends the process inside torch).
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from triturus_amd import _lib
+
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+try:
+    _is_capturing = torch._C._cuda_isCurrentStreamCapturing
+except AttributeError:  # pragma: no cover
+    _is_capturing = torch.cuda.is_current_stream_capturing
+
+
+def refuse_capture(op: str) -> None:
+    if _is_capturing():
+        raise RuntimeError(
+            f"{op}: operands that require a gradient are refused under graph capture; "
+            f"capture {op} on detached operands and {op}_grad"
+        )
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows with a unit trailing stride, in place where the tensor has them."""
+    if t.shape[-1] == 1:
+        return t.as_strided(t.shape, (t.stride(0), 1), t.storage_offset()) if t.stride(0) >= 0 else t.contiguous()
+    return t if t.stride(-1) == 1 and t.stride(0) >= 0 else t.contiguous()
+
+
+def _matrices(b: torch.Tensor) -> torch.Tensor:
+    """Matrices with a unit stride along one of their axes, in place where the tensor has them."""
+    st = b.stride()
+    if min(st) < 0:
+        return b.contiguous()
+    if st[2] == 1 or st[1] == 1:
+        return b
+    if b.shape[2] == 1:
+        return b.as_strided(b.shape, (st[0], st[1], 1), b.storage_offset())
+    if b.shape[1] == 1:
+        return b.as_strided(b.shape, (st[0], 1, st[2]), b.storage_offset())
+    return b.contiguous()
+
+
+def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:
+    assert len(a.shape) == 2 and len(b.shape) == 3 and len(sizes.shape) == 1
+    assert a.shape[1] == b.shape[1]
+    assert b.shape[0] == sizes.shape[0] >= 1
+    assert a.dtype == b.dtype
+    assert sizes.dtype in (torch.int32, torch.int64)
+    assert a.device == b.device == sizes.device
+    if a.dtype not in _TYPES:
+        raise NotImplementedError(f"gmm supports bf16/fp16/fp32, got {a.dtype}")
+    _lib.require_gpu(a, b, sizes)
+
+
+def _forward(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor, tile: int = 0) -> torch.Tensor:
+    T, K = a.shape
+    E, _, N = b.shape
+    c = torch.empty((T, N), dtype=a.dtype, device=a.device)
+    if c.numel() == 0:
+        return c
+    if K == 0:
+        return c.zero_()
+    a, b, sizes = _rows(a), _matrices(b), sizes.contiguous()
+    with _lib.on_device(a.device):
+        status = _lib.load().trt_gmm(
+            a.data_ptr(), b.data_ptr(), sizes.data_ptr(), c.data_ptr(), T, E, K, N, a.stride(0), _lib.strides3(b),
+            _lib.DTYPE_CODES[a.dtype], sizes.dtype == torch.int64, tile, _lib.raw_stream(a.device),
+        )
+    if status:
+        _lib.check(status, "trt_gmm")
+    return c
+
+
+def _weights(a: torch.Tensor, g: torch.Tensor, sizes: torch.Tensor, tile: int = 0) -> torch.Tensor:
+    T, K = a.shape
+    E, N = sizes.shape[0], g.shape[1]
+    d = torch.empty((E, K, N), dtype=a.dtype, device=a.device)
+    if d.numel() == 0:
+        return d
+    if T == 0:
+        return d.zero_()
+    a, g, sizes = _rows(a), _rows(g), sizes.contiguous()
+    with _lib.on_device(a.device):
+        status = _lib.load().trt_gmm_weights(
+            a.data_ptr(), g.data_ptr(), sizes.data_ptr(), d.data_ptr(), T, E, K, N, a.stride(0), g.stride(0),
+            _lib.DTYPE_CODES[a.dtype], sizes.dtype == torch.int64, tile, _lib.raw_stream(a.device),
+        )
+    if status:
+        _lib.check(status, "trt_gmm_weights")
+    return d
+
+
+class _Gmm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, b, sizes):
+        ctx.save_for_backward(a, b, sizes)
+        return _forward(a, b, sizes)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        a, b, sizes = ctx.saved_tensors
+        da = _forward(g, b.transpose(1, 2), sizes) if ctx.needs_input_grad[0] else None
+        db = _weights(a, g, sizes) if ctx.needs_input_grad[1] else None
+        return da, db, None
+
+
+def gmm(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> torch.Tensor:
+    """c[r] = a[r] @ b[e(r)], e(r) the group that row r lies in; zeros behind the last group."""
+    _check(a, b, sizes)
+    if torch.is_grad_enabled() and (a.requires_grad or b.requires_grad):
+        refuse_capture("gmm")
+        return _Gmm.apply(a, b, sizes)
+    return _forward(a, b, sizes)
+
+
+def gmm_grad(g: torch.Tensor, a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gradients (of a, of b) of sum(g * gmm(a, b, sizes)), in the operands' type; zero for rows behind the last group
+    and for matrices of empty groups."""
+    _check(a, b, sizes)
+    assert g.shape == (a.shape[0], b.shape[2])
+    assert g.dtype == a.dtype and g.device == a.device
+    with torch.no_grad():
+        return _forward(g, b.transpose(1, 2), sizes), _weights(a, g, sizes)
