@@ -325,6 +325,30 @@ int trt_gmm_weights(const void *a, const void *g, const void *sizes, void *d, in
                     int64_t N, int64_t lda, int64_t ldg, int dtype, int wide_sizes, int tile, void *stream);
 
 /*
+ * The microscaled 4-bit format (MXFP4 of the OCP Microscaling Formats specification v1.0): blocks of 32 values
+ * along a row share a power of two.  With e = floor(log2 max |x|) - 2, clamped to [-127, 127] and stored as the
+ * byte e + 127, a value is x / 2^e rounded to the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (ties to the even code, beyond 6
+ * to 6) with its sign: 4 bits, sign on top, the even value of a pair in the low half of a byte.  A block with a NaN
+ * or an infinity gets scale 255, which stands for NaN throughout.  A row of K values has ceil(K / 32) blocks of 16
+ * bytes of codes and 1 byte of scale; the last block is filled up with zeros.  No counterpart in the reference.
+ *
+ * trt_mx4_quantize: x (TRT_F32, TRT_F16, TRT_BF16; rows x K, row stride ldx, unit trailing stride) to dense codes
+ * (4-byte aligned) and scales.
+ * trt_mx4_dequantize: back to dense rows of `dtype`, rounded once where its range ends; strides in bytes.
+ * trt_mx4_mm: c[r, n] = sum_k a[r, k] b[e(r), n, k] over the values of both, summed in fp32 and rounded once to
+ * `dtype`.  sizes as for trt_gmm (rows of c behind the last group are zero), or NULL with E = 1: one
+ * matrix for all rows.  a: T rows, sa = {row stride of codes, of scales}; b: E x N rows, sb = {matrix stride of
+ * codes, row stride of codes, matrix stride of scales, row stride of scales}, all in bytes.  Rows of
+ * codes may lie at any address (fastest at multiples of 16 bytes) and at most 8 MiB apart (TRT_E_RANGE).
+ */
+int trt_mx4_quantize(const void *x, void *codes, void *scales, int64_t rows, int64_t K, int64_t ldx, int dtype, void *stream);
+int trt_mx4_dequantize(const void *codes, const void *scales, void *y, int64_t rows, int64_t K, int64_t ld_codes,
+                       int64_t ld_scales, int dtype, void *stream);
+int trt_mx4_mm(const void *a, const void *a_scales, const void *b, const void *b_scales, const void *sizes, void *c,
+               int64_t T, int64_t E, int64_t K, int64_t N, const int64_t sa[2], const int64_t sb[4], int dtype,
+               int wide_sizes, void *stream);
+
+/*
  * r = x + y for contiguous vectors of n elements of `dtype` (TRT_F32 ...).  Replaces the
  * `_ker_vadd[grid](...)` launch, triturus/add.py:45.  Same remark as trt_mm_f32.
  */

@@ -128,8 +128,56 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <typename T>
-__device__ __forceinline__ T round_to(float v) { return (T)v; }
+// Writes a finished tile: `out` is its first value, rows x cols of it exist, the output's rows are N long and start at
+// `base`.  acc[i][j][q] is row 32 i + (lane & 31), column 32 j + 8 (q / 4) + 4 (lane / 32) + q % 4 of the
+// wavefront's part (the MFMA's first operand makes its rows, and that is Y here: 4 neighbours of an output row
+// in a lane).  The wavefront turns them round in LDS of its own and writes rows, 16 bytes a lane.
+template <typename T, int BM, int BN, int WM, int WN>
+struct OutTile {
+    static constexpr int ROW = BN / WN * (int)sizeof(T) + 16;  // bytes of a row of a wavefront's part in LDS
+    static constexpr int LDS = WM * WN * (BM / WM) * ROW;
+};
+
+template <typename T, int BM, int BN, int WM, int WN, int RT, int CT>
+__device__ __forceinline__ void store_tile(const floatx16 (&acc)[RT][CT], char *lds, int wave, T *out, int64_t N, int64_t rows,
+                                           int64_t cols, const void *base) {
+    constexpr int OUT_ROW = OutTile<T, BM, BN, WM, WN>::ROW;
+    const int wm = wave / WN, wn = wave % WN, l = lane_id();
+    char *mine = lds + wave * (BM / WM) * OUT_ROW;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; q += 4) {
+                struct alignas(4 * sizeof(T)) { T v[4]; } four;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) four.v[u] = (T)acc[i][j][q + u];
+                const int row = 32 * i + (l & 31), col = 32 * j + 2 * q + 4 * (l >> 5);
+                *reinterpret_cast<decltype(four) *>(mine + row * OUT_ROW + col * sizeof(T)) = four;
+            }
+    // the wavefront reads what it wrote itself: no barrier
+    constexpr int V = 16 / sizeof(T), PER = BN / WN / V, STEP = kWave / PER;
+    const int64_t wrows = rows - wm * (BM / WM), wcols = cols - wn * (BN / WN);
+    T *dst = out + (int64_t)wm * (BM / WM) * N + wn * (BN / WN);
+    const bool whole = ((reinterpret_cast<uintptr_t>(base) | (uint64_t)(N * (int64_t)sizeof(T))) & 15) == 0;
+    const int c = l % PER * V;
+#pragma unroll 4
+    for (int r = l / PER; r < BM / WM; r += STEP) {
+        if (r >= wrows || c >= wcols) continue;
+        const uintx4 v = *reinterpret_cast<const uintx4 *>(mine + r * OUT_ROW + c * sizeof(T));
+        T *p = dst + (int64_t)r * N + c;
+        if (whole) {
+            *reinterpret_cast<uintx4 *>(p) = v;
+        } else {
+            T e[V];
+            __builtin_memcpy(e, &v, 16);
+#pragma unroll
+            for (int u = 0; u < V; ++u)
+                if (c + u < wcols) p[u] = e[u];
+        }
+    }
+}
 
 struct GmmArgs {
     const void *x, *y;
@@ -147,8 +195,7 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
     using Y = Operand<T, YL, BN, THREADS>;
     constexpr bool WEIGHTS = XL == kOuter;
     constexpr int KT = X::KT, STAGE = X::LDS + Y::LDS;
-    constexpr int OUT_ROW = BN / WN * (int)sizeof(T) + 16;       // bytes of a row of a wavefront's output in LDS
-    constexpr int OUT = WM * WN * (BM / WM) * OUT_ROW;
+    constexpr int OUT = OutTile<T, BM, BN, WM, WN>::LDS;
     __shared__ __attribute__((aligned(16))) char lds[2 * STAGE > OUT ? 2 * STAGE : OUT];
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -232,43 +279,7 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
         lds_barrier();
     }
 
-    // acc[i][j][q] is row 32 i + (lane & 31), column 32 j + 8 (q / 4) + 4 (lane / 32) + q % 4 of the wavefront's part
-    // (the MFMA's first operand makes its rows, and that is Y here: 4 neighbours of an output row in a lane).
-    char *mine = lds + wave * (BM / WM) * OUT_ROW;
-    const int l = lane_id();
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < CT; ++j)
-#pragma unroll
-            for (int q = 0; q < 16; q += 4) {
-                struct alignas(4 * sizeof(T)) { T v[4]; } four;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) four.v[u] = round_to<T>(acc[i][j][q + u]);
-                const int row = 32 * i + (l & 31), col = 32 * j + 2 * q + 4 * (l >> 5);
-                *reinterpret_cast<decltype(four) *>(mine + row * OUT_ROW + col * sizeof(T)) = four;
-            }
-    // the wavefront reads what it wrote itself: no barrier
-    constexpr int V = 16 / sizeof(T), PER = BN / WN / V, STEP = kWave / PER;
-    const int64_t wrows = rows - wm * (BM / WM), wcols = cols - wn * (BN / WN);
-    T *dst = out + (int64_t)wm * (BM / WM) * g.N + wn * (BN / WN);
-    const bool whole = ((reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.N * (int64_t)sizeof(T))) & 15) == 0;
-    const int c = l % PER * V;
-#pragma unroll 4
-    for (int r = l / PER; r < BM / WM; r += STEP) {
-        if (r >= wrows || c >= wcols) continue;
-        const uintx4 v = *reinterpret_cast<const uintx4 *>(mine + r * OUT_ROW + c * sizeof(T));
-        T *p = dst + (int64_t)r * g.N + c;
-        if (whole) {
-            *reinterpret_cast<uintx4 *>(p) = v;
-        } else {
-            T e[V];
-            __builtin_memcpy(e, &v, 16);
-#pragma unroll
-            for (int u = 0; u < V; ++u)
-                if (c + u < wcols) p[u] = e[u];
-        }
-    }
+    store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, g.N, rows, cols, g.out);
 }
 
 }  // namespace trt
