@@ -349,6 +349,25 @@ int trt_mx4_mm(const void *a, const void *a_scales, const void *b, const void *b
                int wide_sizes, void *stream);
 
 /*
+ * The router of a mixture layer.  logits: T x E (TRT_F32, TRT_F16, TRT_BF16; row stride ld, unit trailing stride).  A row
+ * chooses its k largest logits, the lowest index first among equal ones (k <= min(E, 16), E <= 1024, T k < 2^31: TRT_E_RANGE
+ * otherwise); -inf is never chosen (such a choice has expert -1, slot -1 and weight 0), a NaN comes first, as in the max
+ * reductions.  weights: T x k, the softmax of the chosen logits among themselves (normalize != 0) or among all
+ * of the row; a row without a finite choice has zeros.  experts, slots: T x k.  The chosen pairs are ordered by
+ * expert, and by row within an expert: slots is a pair's place, rows (T k values) the row at each place (0
+ * behind the last pair), sizes (E values) the experts' numbers of pairs -- the sizes of trt_gmm.  workspace:
+ * trt_route_workspace_bytes(T, E) bytes, 16-byte aligned, needing no preparation.  No counterpart in the reference.
+ *
+ * trt_route_grad: d = the gradient of sum(g * weights) with respect to the logits, T x E, dense, of their type; g: T x k.
+ */
+int trt_route(const void *logits, float *weights, int32_t *experts, int32_t *rows, int32_t *slots, int32_t *sizes,
+              int64_t T, int64_t E, int64_t k, int64_t ld, int dtype, int normalize, void *workspace,
+              size_t workspace_bytes, void *stream);
+size_t trt_route_workspace_bytes(int64_t T, int64_t E);
+int trt_route_grad(const float *g, const void *logits, const float *weights, const int32_t *experts, void *d, int64_t T,
+                   int64_t E, int64_t k, int64_t ld, int dtype, int normalize, void *stream);
+
+/*
  * r = x + y for contiguous vectors of n elements of `dtype` (TRT_F32 ...).  Replaces the
  * `_ker_vadd[grid](...)` launch, triturus/add.py:45.  Same remark as trt_mm_f32.
  */

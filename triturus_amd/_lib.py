@@ -107,6 +107,16 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
          POINTER(c_int64), POINTER(c_int64), c_int, c_int, c_void_p],
     ),
+    "trt_route": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+         c_int, c_int, c_void_p, c_size_t, c_void_p],
+    ),
+    "trt_route_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "trt_route_grad": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_void_p],
+    ),
     "trt_vadd": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "trt_copy_bytes": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "trt_max_workspace_init": (c_int, [c_void_p, c_size_t, c_void_p]),
