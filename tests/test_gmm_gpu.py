@@ -211,3 +211,17 @@ def test_refusals(dev):
     for bad in (g[:, :3], g.half(), g.cpu()):
         with pytest.raises(AssertionError):
             gmm_grad(bad, a, b, s)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tile", range(1, 5))
+def test_every_tile(dev, tile, dtype):
+    """Each tile on sizes that it would not be chosen for, aligned and not."""
+    from triturus_amd.gmm import _forward, _weights
+
+    for sizes, K, N, tail in (([3, 0, 5, 1], 64, 128, 2), ([33, 0, 64, 65, 31, 2], 129, 77, 11), ([300, 5], 648, 264, 3), ([1] * 70, 40, 8, 0), ([2, 257], 1031, 66, 0)):
+        for layout in ("kn", "nk"):
+            a, b, g = operands(dev, sum(sizes) + tail, len(sizes), K, N, dtype, layout)
+            s = torch.tensor(sizes, device=dev)
+            close(_forward(a, b, s, tile), product64(a, b, sizes), product64(a.abs(), b.abs(), sizes), K)
+            close(_weights(a, g, s, tile), weights64(a, g, sizes), weights64(a.abs(), g.abs(), sizes), max(sizes))
