@@ -340,13 +340,19 @@ int trt_gmm_weights(const void *a, const void *g, const void *sizes, void *d, in
  * matrix for all rows.  a: T rows, sa = {row stride of codes, of scales}; b: E x N rows, sb = {matrix stride of
  * codes, row stride of codes, matrix stride of scales, row stride of scales}, all in bytes.  Rows of
  * codes may lie at any address (fastest at multiples of 16 bytes) and at most 8 MiB apart (TRT_E_RANGE).
+ * a_type: -1 for codes and scales, or TRT_F32, TRT_F16, TRT_BF16 for T x K values that the call quantises
+ * itself (sa[0]: row stride in values; a_scales unused), with a workspace of
+ * trt_mx4_mm_workspace_bytes(T, E, K, a_type, tile) bytes, 16-byte aligned; 0 where the product's kernel quantises
+ * on the way.  tile: 0 = choose by shape, 1..TRT_MX4_TILES force a tile (experiments, tests).
  */
+#define TRT_MX4_TILES 3
 int trt_mx4_quantize(const void *x, void *codes, void *scales, int64_t rows, int64_t K, int64_t ldx, int dtype, void *stream);
 int trt_mx4_dequantize(const void *codes, const void *scales, void *y, int64_t rows, int64_t K, int64_t ld_codes,
                        int64_t ld_scales, int dtype, void *stream);
 int trt_mx4_mm(const void *a, const void *a_scales, const void *b, const void *b_scales, const void *sizes, void *c,
-               int64_t T, int64_t E, int64_t K, int64_t N, const int64_t sa[2], const int64_t sb[4], int dtype,
-               int wide_sizes, void *stream);
+               int64_t T, int64_t E, int64_t K, int64_t N, const int64_t sa[2], const int64_t sb[4], int a_type,
+               int dtype, int wide_sizes, int tile, void *workspace, size_t workspace_bytes, void *stream);
+size_t trt_mx4_mm_workspace_bytes(int64_t T, int64_t E, int64_t K, int a_type, int tile);
 
 /*
  * The router of a mixture layer.  logits: T x E (TRT_F32, TRT_F16, TRT_BF16; row stride ld, unit trailing stride).  A row

@@ -105,8 +105,9 @@ SIGNATURES = {
     "trt_mx4_mm": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
-         POINTER(c_int64), POINTER(c_int64), c_int, c_int, c_void_p],
+         POINTER(c_int64), POINTER(c_int64), c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p],
     ),
+    "trt_mx4_mm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
     "trt_route": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,

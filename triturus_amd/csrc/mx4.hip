@@ -8,7 +8,7 @@
 //
 // Bound: HBM.  A lane takes 16 bytes of the row (32 of fp32), so 4 lanes make a block; the largest is found in 2
 // lane steps and the codes by the conversion instructions, 2 values each.
-#include "grouped.hpp"
+#include "mx4.hpp"
 
 namespace trt {
 
@@ -26,46 +26,6 @@ __device__ __forceinline__ uint32_t divide(uint32_t n, const Divider &v) { retur
 constexpr int kPart = 8;                // values of a lane
 constexpr int kParts = 32 / kPart;      // lanes of a block
 
-template <typename T>
-__device__ __forceinline__ void load_part(const T *p, int64_t left, T (&v)[kPart]) {
-    constexpr int V = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < kPart / V; ++i) {
-        const uintx4 u = load_chunk(p + i * V, left - i * V);
-        __builtin_memcpy(&v[i * V], &u, 16);
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t magnitude(T x) {
-    return __builtin_bit_cast(uint32_t, (float)x) & 0x7fffffffu;
-}
-
-__device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return a > b ? a : b; }
-
-// The lane's 8 codes of a block; `scale` becomes the block's biased exponent.
-template <typename T>
-__device__ __forceinline__ uint32_t quantize_part(const T (&v)[kPart], uint32_t &scale) {
-    uint32_t top = 0;  // as bits: infinities and NaN are above all numbers
-#pragma unroll
-    for (int i = 0; i < kPart; ++i) top = max_u(top, magnitude(v[i]));
-    top = max_u(top, __builtin_amdgcn_mov_dpp(top, 0xB1, 0xf, 0xf, true));  // lanes 1 0 3 2 of each four
-    top = max_u(top, __builtin_amdgcn_mov_dpp(top, 0x4E, 0xf, 0xf, true));  // lanes 2 3 0 1
-    const uint32_t e = top >> 23;
-    scale = e == 255 ? 255 : (e > 2 ? e - 2 : 0);
-    if (scale == 255) return 0;
-    // both factors are normal numbers: x 2^32 / 2^(scale - 127 + 32), exact below 2^96, where it is needed
-    const bool low = scale < 32;
-    const float up = low ? 0x1p32f : 1.0f;
-    const float by = __builtin_bit_cast(float, (scale + (low ? 32 : 0)) << 23);
-    uint32_t codes = 0;
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, (float)v[0] * up, (float)v[1] * up, by, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, (float)v[2] * up, (float)v[3] * up, by, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, (float)v[4] * up, (float)v[5] * up, by, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, (float)v[6] * up, (float)v[7] * up, by, 3);
-    return codes;
-}
-
 // x: rows of K values, row stride ld; codes: rows of 16 * blocks bytes, scales: rows of `blocks` bytes, both dense.
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T *__restrict__ x, uint32_t *__restrict__ codes,
@@ -75,9 +35,12 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T *__restrict__
     if (i >= parts) return;  // blocks end with a group of four lanes
     const uint32_t row = divide(i, per_row), at = i - row * per_row.d;
     T v[kPart];
-    load_part(x + row * ld + at * kPart, K - (int64_t)at * kPart, v);
-    uint32_t scale;
-    codes[i] = quantize_part(v, scale);
+    load_values(x + row * ld + at * kPart, K - (int64_t)at * kPart, v);
+    uint32_t top = top_bits(v);
+    top = max_u(top, __builtin_amdgcn_mov_dpp(top, 0xB1, 0xf, 0xf, true));  // lanes 1 0 3 2 of each four
+    top = max_u(top, __builtin_amdgcn_mov_dpp(top, 0x4E, 0xf, 0xf, true));  // lanes 2 3 0 1
+    const uint32_t scale = block_scale(top);
+    codes[i] = codes_of(v, scale);
     if (i % kParts == 0) scales[i / kParts] = (uint8_t)scale;
 }
 

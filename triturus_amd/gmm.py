@@ -42,50 +42,52 @@ def refuse_capture(op: str) -> None:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Rows with a unit trailing stride, in place where the tensor has them."""
-    if t.shape[-1] == 1:
-        return t.as_strided(t.shape, (t.stride(0), 1), t.storage_offset()) if t.stride(0) >= 0 else t.contiguous()
-    return t if t.stride(-1) == 1 and t.stride(0) >= 0 else t.contiguous()
+    st = t.stride()
+    return t if (st[1] == 1 or t.shape[1] == 1) and st[0] >= 0 else t.contiguous()
 
 
 def _matrices(b: torch.Tensor) -> torch.Tensor:
     """Matrices with a unit stride along one of their axes, in place where the tensor has them."""
     st = b.stride()
-    if min(st) < 0:
-        return b.contiguous()
-    if st[2] == 1 or st[1] == 1:
+    if (st[2] == 1 or st[1] == 1) and min(st) >= 0:
         return b
-    if b.shape[2] == 1:
-        return b.as_strided(b.shape, (st[0], st[1], 1), b.storage_offset())
-    if b.shape[1] == 1:
-        return b.as_strided(b.shape, (st[0], 1, st[2]), b.storage_offset())
+    if min(st) >= 0:
+        if b.shape[2] == 1:
+            return b.as_strided(b.shape, (st[0], st[1], 1), b.storage_offset())
+        if b.shape[1] == 1:
+            return b.as_strided(b.shape, (st[0], 1, st[2]), b.storage_offset())
     return b.contiguous()
 
 
 def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:
-    assert len(a.shape) == 2 and len(b.shape) == 3 and len(sizes.shape) == 1
-    assert a.shape[1] == b.shape[1]
-    assert b.shape[0] == sizes.shape[0] >= 1
-    assert a.dtype == b.dtype
+    sa, sb, ss = a.shape, b.shape, sizes.shape
+    assert len(sa) == 2 and len(sb) == 3 and len(ss) == 1
+    assert sa[1] == sb[1]
+    assert sb[0] == ss[0] >= 1
+    dtype = a.dtype
+    assert dtype is b.dtype
     assert sizes.dtype in (torch.int32, torch.int64)
-    assert a.device == b.device == sizes.device
-    if a.dtype not in _TYPES:
-        raise NotImplementedError(f"gmm supports bf16/fp16/fp32, got {a.dtype}")
-    _lib.require_gpu(a, b, sizes)
+    dev = a.device
+    assert dev == b.device and dev == sizes.device
+    if dtype not in _TYPES:
+        raise NotImplementedError(f"gmm supports bf16/fp16/fp32, got {dtype}")
+    _lib.require_gpu(a)
 
 
 def _forward(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor, tile: int = 0) -> torch.Tensor:
     T, K = a.shape
     E, _, N = b.shape
-    c = torch.empty((T, N), dtype=a.dtype, device=a.device)
-    if c.numel() == 0:
+    dtype, dev = a.dtype, a.device
+    c = torch.empty((T, N), dtype=dtype, device=dev)
+    if T == 0 or N == 0:
         return c
     if K == 0:
         return c.zero_()
     a, b, sizes = _rows(a), _matrices(b), sizes.contiguous()
-    with _lib.on_device(a.device):
+    with _lib.on_device(dev):
         status = _lib.load().trt_gmm(
             a.data_ptr(), b.data_ptr(), sizes.data_ptr(), c.data_ptr(), T, E, K, N, a.stride(0), _lib.strides3(b),
-            _lib.DTYPE_CODES[a.dtype], sizes.dtype == torch.int64, tile, _lib.raw_stream(a.device),
+            _lib.DTYPE_CODES[dtype], sizes.dtype is torch.int64, tile, _lib.raw_stream(dev),
         )
     if status:
         _lib.check(status, "trt_gmm")
@@ -95,16 +97,17 @@ def _forward(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor, tile: int = 
 def _weights(a: torch.Tensor, g: torch.Tensor, sizes: torch.Tensor, tile: int = 0) -> torch.Tensor:
     T, K = a.shape
     E, N = sizes.shape[0], g.shape[1]
-    d = torch.empty((E, K, N), dtype=a.dtype, device=a.device)
+    dtype, dev = a.dtype, a.device
+    d = torch.empty((E, K, N), dtype=dtype, device=dev)
     if d.numel() == 0:
         return d
     if T == 0:
         return d.zero_()
     a, g, sizes = _rows(a), _rows(g), sizes.contiguous()
-    with _lib.on_device(a.device):
+    with _lib.on_device(dev):
         status = _lib.load().trt_gmm_weights(
             a.data_ptr(), g.data_ptr(), sizes.data_ptr(), d.data_ptr(), T, E, K, N, a.stride(0), g.stride(0),
-            _lib.DTYPE_CODES[a.dtype], sizes.dtype == torch.int64, tile, _lib.raw_stream(a.device),
+            _lib.DTYPE_CODES[dtype], sizes.dtype is torch.int64, tile, _lib.raw_stream(dev),
         )
     if status:
         _lib.check(status, "trt_gmm_weights")
@@ -129,7 +132,7 @@ class _Gmm(torch.autograd.Function):
 def gmm(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> torch.Tensor:
     """c[r] = a[r] @ b[e(r)], e(r) the group that row r lies in; zeros behind the last group."""
     _check(a, b, sizes)
-    if torch.is_grad_enabled() and (a.requires_grad or b.requires_grad):
+    if (a.requires_grad or b.requires_grad) and torch.is_grad_enabled():
         refuse_capture("gmm")
         return _Gmm.apply(a, b, sizes)
     return _forward(a, b, sizes)

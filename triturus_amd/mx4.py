@@ -46,40 +46,47 @@ def _type_code(dtype: torch.dtype, op: str) -> int:
 
 
 def _check(q: MX4) -> None:
-    blocks = -(-q.length // BLOCK)
-    assert q.length >= 0
-    assert q.codes.dtype == q.scales.dtype == torch.uint8
-    assert len(q.codes.shape) >= 1 and q.codes.shape[:-1] == q.scales.shape[:-1]
-    assert q.codes.shape[-1] == 16 * blocks and q.scales.shape[-1] == blocks
-    assert q.codes.device == q.scales.device
-    _lib.require_gpu(q.codes, q.scales)
+    codes, scales, length = q
+    shape, blocks = codes.shape, -(-length // BLOCK)
+    assert length >= 0
+    assert codes.dtype is torch.uint8 and scales.dtype is torch.uint8
+    assert len(shape) >= 1 and shape[-1] == 16 * blocks
+    assert scales.shape == (*shape[:-1], blocks)
+    assert codes.device == scales.device
+    _lib.require_gpu(codes)
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:
     """Bytes of a row next to each other, in place where they are."""
     st = t.stride()
-    if min(st) >= 0 and (st[-1] == 1 or t.shape[-1] == 1):
+    if (st[-1] == 1 or t.shape[-1] == 1) and min(st) >= 0:
         return t
     return t.contiguous()
 
 
+def _values(x: torch.Tensor) -> torch.Tensor:
+    """Rows of values with a unit trailing stride, in place where the tensor has them."""
+    st = x.stride()
+    return x if (st[1] == 1 or x.shape[1] == 1) and st[0] >= 0 else x.contiguous()
+
+
 def mx4_quantize(x: torch.Tensor) -> MX4:
     """The 4-bit form of x along its last axis."""
-    assert len(x.shape) >= 1
+    shape = x.shape
+    assert len(shape) >= 1
     code = _type_code(x.dtype, "mx4_quantize")
     _lib.require_gpu(x)
-    K = x.shape[-1]
+    K, dev = shape[-1], x.device
     blocks = -(-K // BLOCK)
-    codes = torch.empty((*x.shape[:-1], 16 * blocks), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=x.device)
+    codes = torch.empty((*shape[:-1], 16 * blocks), dtype=torch.uint8, device=dev)
+    scales = torch.empty((*shape[:-1], blocks), dtype=torch.uint8, device=dev)
     if codes.numel() == 0:
         return MX4(codes, scales, K)
-    flat = x.detach().reshape(-1, K)
-    if K > 1 and flat.stride(1) != 1 or flat.stride(0) < 0:
-        flat = flat.contiguous()
-    with _lib.on_device(x.device):
-        status = _lib.load().trt_mx4_quantize(flat.data_ptr(), codes.data_ptr(), scales.data_ptr(), flat.shape[0], K,
-                                              flat.stride(0), code, _lib.raw_stream(x.device))
+    x = x.detach() if x.requires_grad else x
+    x = _values(x if len(shape) == 2 else x.reshape(-1, K))
+    with _lib.on_device(dev):
+        status = _lib.load().trt_mx4_quantize(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.shape[0], K, x.stride(0), code,
+                                              _lib.raw_stream(dev))
     if status:
         _lib.check(status, "trt_mx4_quantize")
     return MX4(codes, scales, K)
@@ -89,54 +96,83 @@ def mx4_dequantize(q: MX4, *, dtype: torch.dtype = torch.float32) -> torch.Tenso
     """The values that q stands for (exact in fp32, and in bf16 unless its exponent range ends)."""
     _check(q)
     code = _type_code(dtype, "mx4_dequantize")
-    y = torch.empty((*q.codes.shape[:-1], q.length), dtype=dtype, device=q.codes.device)
+    codes, scales, K = q
+    shape, dev = codes.shape, codes.device
+    y = torch.empty((*shape[:-1], K), dtype=dtype, device=dev)
     if y.numel() == 0:
         return y
-    codes, scales = _unit(q.codes.reshape(-1, q.codes.shape[-1])), _unit(q.scales.reshape(-1, q.scales.shape[-1]))
-    with _lib.on_device(y.device):
-        status = _lib.load().trt_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), codes.shape[0], q.length,
-                                                codes.stride(0), scales.stride(0), code, _lib.raw_stream(y.device))
+    if len(shape) != 2:
+        codes, scales = codes.reshape(-1, shape[-1]), scales.reshape(-1, scales.shape[-1])
+    codes, scales = _unit(codes), _unit(scales)
+    with _lib.on_device(dev):
+        status = _lib.load().trt_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), codes.shape[0], K,
+                                                codes.stride(0), scales.stride(0), code, _lib.raw_stream(dev))
     if status:
         _lib.check(status, "trt_mx4_dequantize")
     return y
 
 
-def mm_mx4(a: torch.Tensor | MX4, b: MX4, sizes: torch.Tensor | None = None, *, dtype: torch.dtype | None = None) -> torch.Tensor:
-    """c[r, n] = sum_k a[r, k] b[n, k], or with ``sizes`` b[e(r), n, k]; ``dtype``: of c, by default a's (bf16 for an MX4)."""
-    if not isinstance(a, MX4):
-        assert len(a.shape) == 2
-        dtype = dtype or a.dtype
-        _type_code(a.dtype, "mm_mx4")
+_ws_bytes: dict = {}  # (T, E, K, type of a) -> workspace bytes, as reported by the library
+
+
+def mm_mx4(a: torch.Tensor | MX4, b: MX4, sizes: torch.Tensor | None = None, *, dtype: torch.dtype | None = None,
+           _tile: int = 0) -> torch.Tensor:
+    """c[r, n] = sum_k a[r, k] b[n, k], or with ``sizes`` b[e(r), n, k]; ``dtype``: of c, by default a's (bf16 for an MX4).
+
+    ``_tile`` forces a kernel (tests, timing)."""
+    _check(b)
+    bc, bs, K = b
+    shape = bc.shape
+    if isinstance(a, MX4):
+        _check(a)
+        assert len(a.codes.shape) == 2 and a.length == K
+        ac, as_, a_type = _unit(a.codes), _unit(a.scales), -1
+        dtype = dtype or torch.bfloat16
+        sa = _I64x2(ac.stride(0), as_.stride(0))
+    else:
+        assert len(a.shape) == 2 and a.shape[1] == K
+        a_type = _type_code(a.dtype, "mm_mx4")
         if a.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("mm_mx4 has no gradient: detach its operand")
-        a = mx4_quantize(a)
-    dtype = dtype or torch.bfloat16
+        ac = as_ = _values(a)
+        dtype = dtype or a.dtype
+        sa = _I64x2(ac.stride(0), 0)
     code = _type_code(dtype, "mm_mx4")
-    _check(a)
-    _check(b)
-    assert len(a.codes.shape) == 2 and len(b.codes.shape) == (2 if sizes is None else 3)
-    assert a.length == b.length
-    assert a.codes.device == b.codes.device
-    T, N, K = a.codes.shape[0], b.codes.shape[-2], a.length
-    E = 1 if sizes is None else b.codes.shape[0]
-    if sizes is not None:
-        assert len(sizes.shape) == 1 and sizes.shape[0] == E >= 1
-        assert sizes.dtype in (torch.int32, torch.int64)
-        assert sizes.device == a.codes.device
+    dev = ac.device
+    assert dev == bc.device
+    T, N = ac.shape[0], shape[-2] if len(shape) > 1 else 0
+    if sizes is None:
+        assert len(shape) == 2
+        E, wide, sizes_ptr = 1, False, None
+    else:
+        assert len(shape) == 3 and len(sizes.shape) == 1
+        E, wide = shape[0], sizes.dtype is torch.int64
+        assert sizes.shape[0] == E >= 1
+        assert wide or sizes.dtype is torch.int32
+        assert sizes.device == dev
         sizes = sizes.contiguous()
-    c = torch.empty((T, N), dtype=dtype, device=a.codes.device)
-    if c.numel() == 0:
+        sizes_ptr = sizes.data_ptr()
+    c = torch.empty((T, N), dtype=dtype, device=dev)
+    if T == 0 or N == 0:
         return c
     if K == 0:
         return c.zero_()
-    ac, as_, bc, bs = _unit(a.codes), _unit(a.scales), _unit(b.codes), _unit(b.scales)
-    with _lib.on_device(c.device):
-        status = _lib.load().trt_mx4_mm(
-            ac.data_ptr(), as_.data_ptr(), bc.data_ptr(), bs.data_ptr(), None if sizes is None else sizes.data_ptr(), c.data_ptr(),
-            T, E, K, N, _I64x2(ac.stride(0), as_.stride(0)),
-            _I64x4(0 if sizes is None else bc.stride(0), bc.stride(-2), 0 if sizes is None else bs.stride(0), bs.stride(-2)),
-            code, sizes is not None and sizes.dtype == torch.int64, _lib.raw_stream(c.device),
-        )
+    bc, bs = _unit(bc), _unit(bs)
+    lib = _lib.load()
+    nbytes = 0
+    if a_type >= 0:
+        key = (T, E, K, a_type, _tile)
+        nbytes = _ws_bytes.get(key)
+        if nbytes is None:
+            if len(_ws_bytes) > 4096:
+                _ws_bytes.clear()
+            nbytes = _ws_bytes[key] = lib.trt_mx4_mm_workspace_bytes(*key)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    cst, sst = bc.stride(), bs.stride()
+    sb = _I64x4(0, cst[0], 0, sst[0]) if sizes is None else _I64x4(cst[0], cst[1], sst[0], sst[1])
+    with _lib.on_device(dev):
+        status = lib.trt_mx4_mm(ac.data_ptr(), as_.data_ptr(), bc.data_ptr(), bs.data_ptr(), sizes_ptr, c.data_ptr(), T, E, K, N, sa, sb,
+                                a_type, code, wide, _tile, ws.data_ptr() if nbytes else None, nbytes, _lib.raw_stream(dev))
     if status:
         _lib.check(status, "trt_mx4_mm")
     return c

@@ -56,13 +56,12 @@ def _route(logits: torch.Tensor, k: int, normalize: bool) -> Routes:
     code = _check(logits, k)
     T, E = logits.shape
     dev = logits.device
-    out = Routes(
-        torch.empty((T, k), dtype=torch.float32, device=dev), torch.empty((T, k), dtype=torch.int32, device=dev),
-        torch.empty(T * k, dtype=torch.int32, device=dev), torch.empty((T, k), dtype=torch.int32, device=dev),
-        torch.empty(E, dtype=torch.int32, device=dev),
-    )
+    # one allocation for the four T x k results: they come and go together, and a small call is bound by the host
+    weights, experts, rows, slots = torch.empty((4, T, k), dtype=torch.int32, device=dev).unbind(0)
+    sizes = torch.empty(E, dtype=torch.int32, device=dev)
+    out = Routes(weights.view(torch.float32), experts, rows.view(-1), slots, sizes)
     if T == 0:
-        out.sizes.zero_()
+        sizes.zero_()
         return out
     logits = _rows(logits)
     lib = _lib.load()
@@ -70,7 +69,7 @@ def _route(logits: torch.Tensor, k: int, normalize: bool) -> Routes:
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _lib.on_device(dev):
         status = lib.trt_route(
-            logits.data_ptr(), *(t.data_ptr() for t in out), T, E, k, logits.stride(0), code, int(bool(normalize)),
+            logits.data_ptr(), weights.data_ptr(), experts.data_ptr(), rows.data_ptr(), slots.data_ptr(), sizes.data_ptr(), T, E, k, logits.stride(0), code, int(bool(normalize)),
             ws.data_ptr() if nbytes else None, nbytes, _lib.raw_stream(dev),
         )
     if status:
@@ -111,7 +110,7 @@ class _Route(torch.autograd.Function):
 
 def route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Routes:
     """The k largest logits of every row, their weights, and the pairs ordered by expert."""
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         _check(logits, k)
         refuse_capture("route")
         return Routes(*_Route.apply(logits, k, normalize))
