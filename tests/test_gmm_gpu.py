@@ -214,7 +214,7 @@ def test_refusals(dev):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("tile", range(1, 5))
+@pytest.mark.parametrize("tile", range(1, 6))
 def test_every_tile(dev, tile, dtype):
     """Each tile on sizes that it would not be chosen for, aligned and not."""
     from triturus_amd.gmm import _forward, _weights

@@ -243,7 +243,7 @@ def test_refusals(dev):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("tile", range(1, 4))
+@pytest.mark.parametrize("tile", range(1, 5))
 def test_every_tile(dev, tile, dtype):
     """Each tile on sizes that it would not be chosen for; values quantised within the call and before are the same bits."""
     for sizes, K, N, tail in (([3, 0, 5, 1], 64, 128, 2), ([33, 0, 64, 65, 31, 2], 130, 77, 11), ([300, 5], 2048, 264, 3), ([1] * 70, 40, 8, 0), ([150], 3000, 66, 0)):

@@ -121,6 +121,27 @@ __global__ __launch_bounds__(64 * kFewWaves) void gmm_few_kernel(GmmArgs g) {
                     }
                 }
             }
+        } else if (k0 + KT <= terms && (YL == kInner || cols >= kFewCols)) {
+            // every chunk is whole; a row or column that does not exist is read as the last one that does, and never written
+            const int rlast = rows < 16 * RT ? (int)rows - 1 : 16 * RT - 1, clast = cols < kFewCols ? (int)cols - 1 : kFewCols - 1;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const int r = 16 * i + m < rlast ? 16 * i + m : rlast;
+                __builtin_memcpy(&n.x[i], xp + r * g.ldx + gk * V, 16);
+            }
+#pragma unroll
+            for (int i = 0; i < (YL == kInner ? 4 : V); ++i) {
+                if constexpr (YL == kInner) {
+                    const int c = 16 * i + m < clast ? 16 * i + m : clast;
+                    __builtin_memcpy(&n.y[i], yp + c * g.ldy + gk * V, 16);
+                } else if constexpr (sizeof(T) == 4) {
+                    __builtin_memcpy(&n.y[i], yp + (gk * V + i) * g.ldy + 4 * m, 16);
+                } else {
+                    uintx2 v;
+                    __builtin_memcpy(&v, yp + (gk * V + i) * g.ldy + 4 * m, 8);
+                    n.y[i / 2][i % 2 * 2] = v[0], n.y[i / 2][i % 2 * 2 + 1] = v[1];
+                }
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < RT; ++i) n.x[i] = load_chunk(xp + (16 * i + m) * g.ldx + gk * V, 16 * i + m < rows ? left : 0);

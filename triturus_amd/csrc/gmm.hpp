@@ -18,11 +18,14 @@
 // written 16 bytes a lane.
 #pragma once
 
+#include <utility>
+
 #include "grouped.hpp"
 
 namespace trt {
 
 enum { kInner = 0, kOuter = 1 };
+constexpr int kStepBytes = 64, kStages = 3, kSub = kStepBytes / 32;  // sub-steps: MFMAs of 32 bytes per row
 
 template <typename T>
 struct Mfma;
@@ -52,13 +55,17 @@ struct Mfma<float> {
 template <typename T, int LAYOUT, int B, int THREADS>
 struct Operand {
     static constexpr int V = 16 / sizeof(T);           // values per chunk
-    static constexpr int KT = 128 / sizeof(T);         // contracted values per step
-    static constexpr int ROW = LAYOUT == kInner ? 128 : B * (int)sizeof(T) + 32;  // bytes of an LDS row
-    static constexpr int LDS = LAYOUT == kInner ? B * 128 : KT * ROW;
-    static constexpr int PER_ROW = LAYOUT == kInner ? 8 : B / V;  // chunks per LDS row
-    static constexpr int N = B * 8 / THREADS;          // chunks per thread
+    static constexpr int KT = kStepBytes / sizeof(T);  // contracted values per step
+    static constexpr int CHUNKS = kStepBytes / 16;
+    static constexpr int ROW = LAYOUT == kInner ? kStepBytes : B * (int)sizeof(T) + 32;  // bytes of an LDS row
+    static constexpr int LDS = LAYOUT == kInner ? B * kStepBytes : KT * ROW;
+    static constexpr int PER_ROW = LAYOUT == kInner ? CHUNKS : B / V;  // chunks per LDS row
+    static constexpr int N = B * CHUNKS / THREADS;     // chunks per thread
     static constexpr int ROWS_STEP = THREADS / PER_ROW;
-    static_assert(THREADS % PER_ROW == 0 && B * 8 % THREADS == 0, "threads cover whole LDS rows");
+    static_assert(THREADS % PER_ROW == 0 && B * CHUNKS % THREADS == 0, "threads cover whole LDS rows");
+
+    // INNER: chunk c of row r lies at c ^ (r / 2 % 4), so that 8 neighbouring rows' chunks c lie in different banks
+    static __device__ __forceinline__ int place(int row, int c) { return row * ROW + ((c ^ ((row >> 1) & 3)) * 16); }
 
     uintx4 reg[N];
 
@@ -77,6 +84,14 @@ struct Operand {
                 const uint32_t at = in > 0 && row < rows ? row * row_bytes + (uint32_t)(c * sizeof(T)) : 0x80000000u;
                 reg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0);
             }
+        } else if (left >= KT && (LAYOUT == kInner || out >= B)) {
+            // every chunk is whole; a row of the tile that does not exist is read as the last one that does, and never written
+            const int last = LAYOUT == kInner && out < B ? (int)out - 1 : (LAYOUT == kInner ? B : KT) - 1;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int row = r + i * ROWS_STEP;
+                __builtin_memcpy(&reg[i], p + (row < last ? row : last) * ld + c, 16);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -91,17 +106,16 @@ struct Operand {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int row = r + i * ROWS_STEP;
-            const int at = LAYOUT == kInner ? row * ROW + ((c ^ (row & 7)) * 16) : row * ROW + c * 16;
+            const int at = LAYOUT == kInner ? place(row, c) : row * ROW + c * 16;
             *reinterpret_cast<uintx4 *>(lds + at) = reg[i];
         }
     }
 
-    // The lane's 16 bytes for sub-step kk (0..3) and the 32 rows from `row` on: contracted chunk 2 kk + (lane >= 32).
+    // The lane's 16 bytes for sub-step kk and the 32 rows from `row` on: contracted chunk 2 kk + (lane >= 32).
     static __device__ __forceinline__ uintx4 fragment(const char *lds, int row, int kk) {
         const int l = lane_id(), half = l >> 5, m = l & 31;
         if constexpr (LAYOUT == kInner) {
-            const int rr = row + m;
-            return *reinterpret_cast<const uintx4 *>(lds + rr * ROW + (((2 * kk + half) ^ (rr & 7)) * 16));
+            return *reinterpret_cast<const uintx4 *>(lds + place(row + m, 2 * kk + half));
         } else if constexpr (sizeof(T) == 2) {
             typedef short short4v __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) short4v *lds4;
@@ -179,6 +193,23 @@ __device__ __forceinline__ void store_tile(const floatx16 (&acc)[RT][CT], char *
     }
 }
 
+// Asks the scheduler for the block's instructions in turn: LDS writes, loads, LDS reads, MFMAs, an eighth of each at a time.
+template <int WRITES, int READS, int MFMAS, int... Q>
+__device__ __forceinline__ void interleave(std::integer_sequence<int, Q...>) {
+    constexpr int G = sizeof...(Q);
+    auto part = [](auto q) {
+        constexpr int i = decltype(q)::value;
+        constexpr int w = WRITES * (i + 1) / G - WRITES * i / G, r = READS * (i + 1) / G - READS * i / G, m = MFMAS * (i + 1) / G - MFMAS * i / G;
+        if constexpr (w > 0) {
+            __builtin_amdgcn_sched_group_barrier(0x200, w, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, w, 0);
+        }
+        if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
+        if constexpr (m > 0) __builtin_amdgcn_sched_group_barrier(0x008, m, 0);
+    };
+    (part(std::integral_constant<int, Q>()), ...);
+}
+
 struct GmmArgs {
     const void *x, *y;
     void *out;
@@ -188,46 +219,26 @@ struct GmmArgs {
     uint32_t row_tiles, columns;  // weights: tiles of a matrix
 };
 
+// LDS of a tile: the stages, or the finished tile.
+template <typename T, int XL, int YL, int BM, int BN, int WM, int WN>
+struct GmmLds {
+    static constexpr int THREADS = 64 * WM * WN;
+    static constexpr int STAGE = Operand<T, XL, BM, THREADS>::LDS + Operand<T, YL, BN, THREADS>::LDS;
+    static constexpr int OUT = OutTile<T, BM, BN, WM, WN>::LDS;
+    static constexpr int BYTES = kStages * STAGE > OUT ? kStages * STAGE : OUT;
+};
+
+// One tile: x, y and out at its first values, rows x cols of it exist, `terms` contracted values; `base`: where out's rows of N
+// start.
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED>
-__global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
+__device__ __forceinline__ void gmm_tile(const T *x, int64_t ldx, const T *y, int64_t ldy, T *out, int64_t N, int64_t rows, int64_t cols,
+                                         int64_t terms, const void *base, char *lds) {
     constexpr int THREADS = 64 * WM * WN, RT = BM / WM / 32, CT = BN / WN / 32;
     using X = Operand<T, XL, BM, THREADS>;
     using Y = Operand<T, YL, BN, THREADS>;
-    constexpr bool WEIGHTS = XL == kOuter;
     constexpr int KT = X::KT, STAGE = X::LDS + Y::LDS;
-    constexpr int OUT = OutTile<T, BM, BN, WM, WN>::LDS;
-    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE > OUT ? 2 * STAGE : OUT];
-
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const T *x = static_cast<const T *>(g.x), *y = static_cast<const T *>(g.y);
-    T *out = static_cast<T *>(g.out);
-    int64_t rows, terms;  // of the tile that exist; of the contraction
-    int64_t col0;
-    if constexpr (WEIGHTS) {
-        const uint32_t per = g.row_tiles * g.columns;
-        const uint32_t id = (uint32_t)xcd_logical_id(blockIdx.x, gridDim.x);
-        const uint32_t e = id / per, in = id % per;
-        if (e >= g.sizes.E) return;
-        const int64_t m0 = (int64_t)(in % g.row_tiles) * BM;
-        col0 = (int64_t)(in / g.row_tiles) * BN;
-        int64_t row0;
-        group_rows(g.sizes, e, row0, terms);
-        x += row0 * g.ldx + m0;
-        y += row0 * g.ldy + col0;
-        rows = g.M - m0;
-        out += (e * g.M + m0) * g.N + col0;
-    } else {
-        GroupTile t;
-        if (!find_tile<BM>(g.sizes, blockIdx.x, g.columns, t)) return;
-        col0 = t.column * BN;
-        rows = t.rows;
-        terms = t.group < g.sizes.E ? g.K : 0;  // behind the last group: zeros
-        x += t.row0 * g.ldx;
-        y += (t.group < g.sizes.E ? t.group : 0) * g.y_group + col0 * (YL == kInner ? g.ldy : 1);
-        out += t.row0 * g.N + col0;
-    }
-    const int64_t cols = g.N - col0;
-    const int64_t x_step = XL == kInner ? KT : KT * g.ldx, y_step = YL == kInner ? KT : KT * g.ldy;
+    const int64_t x_step = XL == kInner ? KT : KT * ldx, y_step = YL == kInner ? KT : KT * ldy;
 
     floatx16 acc[RT][CT];
 #pragma unroll
@@ -242,44 +253,109 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
     Y ys;
     const int64_t steps = ceil_div(terms, KT);
     if (steps > 0) {
-        xs.template load<ALIGNED>(x, g.ldx, rows, terms, tid);
-        ys.template load<ALIGNED>(y, g.ldy, cols, terms, tid);
-        xs.store(lds, tid);
-        ys.store(lds + X::LDS, tid);
-        if (steps > 1) {
-            xs.template load<ALIGNED>(x + x_step, g.ldx, rows, terms - KT, tid);
-            ys.template load<ALIGNED>(y + y_step, g.ldy, cols, terms - KT, tid);
-        }
+        auto load = [&](int64_t s) {  // behind the last step nothing remains, and nothing is read
+            const int64_t left = terms - s * KT;
+            xs.template load<ALIGNED>(x + s * x_step, ldx, rows, left, tid);
+            ys.template load<ALIGNED>(y + s * y_step, ldy, cols, left, tid);
+        };
+        auto store = [&](char *to) {
+            xs.store(to, tid);
+            ys.store(to + X::LDS, tid);
+        };
+        uintx4 xf[2][RT], yf[2][CT];
+        auto fragments = [&](const char *from, int kk) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) xf[kk & 1][i] = X::fragment(from, (wm * RT + i) * 32, kk);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) yf[kk & 1][j] = Y::fragment(from + X::LDS, (wn * CT + j) * 32, kk);
+        };
+        load(0);
+        store(lds);
+        load(1);
+        store(lds + STAGE);
+        load(2);
         lds_barrier();
-    }
-    for (int64_t s = 0; s < steps; ++s) {
-        const char *xl = lds + (s & 1) * STAGE, *yl = xl + X::LDS;
-        char *next = lds + ((s + 1) & 1) * STAGE;
+        fragments(lds, 0);
+        char *now = lds, *next = lds + STAGE, *after = lds + 2 * STAGE;
+        for (int64_t s = 0; s < steps; ++s) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            uintx4 xf[RT], yf[CT];
+            for (int kk = 0; kk < kSub; ++kk) {
+                constexpr int MF = sizeof(T) == 4 ? 4 : 1;  // MFMAs of a product of fragments
+                constexpr int XR = XL == kInner ? 1 : sizeof(T) == 2 ? 2 : 4, YR = YL == kInner ? 1 : sizeof(T) == 2 ? 2 : 4;
+                constexpr int READS = RT * XR + CT * YR, MFMAS = RT * CT * MF;
+                if (kk == kSub - 1) {
+                    store(after);  // the step that was read last: everyone is past the barrier behind it
+                    load(s + 3);
+                    fragments(next, 0);
+                } else {
+                    fragments(now, kk + 1);
+                }
 #pragma unroll
-            for (int i = 0; i < RT; ++i) xf[i] = X::fragment(xl, (wm * RT + i) * 32, kk);
+                for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int j = 0; j < CT; ++j) yf[j] = Y::fragment(yl, (wn * CT + j) * 32, kk);
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int j = 0; j < CT; ++j) acc[i][j] = Mfma<T>::step(yf[j], xf[i], acc[i][j]);
-            if (kk == 0 && s + 1 < steps) {
-                xs.store(next, tid);
-                ys.store(next + X::LDS, tid);
-                if (s + 2 < steps) {
-                    const int64_t left = terms - (s + 2) * KT;
-                    xs.template load<ALIGNED>(x + (s + 2) * x_step, g.ldx, rows, left, tid);
-                    ys.template load<ALIGNED>(y + (s + 2) * y_step, g.ldy, cols, left, tid);
+                    for (int j = 0; j < CT; ++j) acc[i][j] = Mfma<T>::step(yf[kk & 1][j], xf[kk & 1][i], acc[i][j]);
+                if constexpr (ALIGNED) {
+                    if (kk == kSub - 1) interleave<X::N + Y::N, READS, MFMAS>(std::make_integer_sequence<int, 8>());
+                    else interleave<0, READS, MFMAS>(std::make_integer_sequence<int, 8>());
                 }
             }
+            lds_barrier();
+            char *const read = now;
+            now = next, next = after, after = read;
         }
-        lds_barrier();
     }
+    store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, N, rows, cols, base);
+}
 
-    store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, g.N, rows, cols, g.out);
+// CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
+template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT>
+__global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
+    static_assert(!CUT || (BM == 256 && BN == 256 && WM == 2 && WN == 4 && XL == kInner), "the parts below");
+    __shared__ __attribute__((aligned(16))) char lds[GmmLds<T, XL, YL, BM, BN, WM, WN>::BYTES];
+    const T *x = static_cast<const T *>(g.x), *y = static_cast<const T *>(g.y);
+    T *out = static_cast<T *>(g.out);
+    if constexpr (XL == kOuter) {
+        // Groups differ in length: each one's tiles are dealt out to all XCDs, in runs of neighbours and in bands of 8 row
+        // tiles (a run shares panels of both operands in its XCD's L2).  The first run goes to another XCD from
+        // group to group, so that matrices of few tiles fill all XCDs too.  (8 groups of 2048 rows on average, K = N = 4096: 1390 us
+        // with a group per XCD, 680 us so.)
+        const uint32_t per = g.row_tiles * g.columns, run = (per + kXcds - 1) / kXcds;
+        const uint32_t e = blockIdx.x / kXcds / run;
+        const uint32_t in = (blockIdx.x + e) % kXcds * run + blockIdx.x / kXcds % run;
+        if (in >= per) return;
+        constexpr uint32_t kBand = 8;
+        const uint32_t band = in / (kBand * g.columns), in_band = in - band * kBand * g.columns;
+        const uint32_t high = g.row_tiles - band * kBand < kBand ? g.row_tiles - band * kBand : kBand;
+        const int64_t m0 = (int64_t)(band * kBand + in_band % high) * BM, col0 = (int64_t)(in_band / high) * BN;
+        int64_t row0, terms;
+        group_rows(g.sizes, e, row0, terms);
+        gmm_tile<T, XL, YL, BM, BN, WM, WN, ALIGNED>(x + row0 * g.ldx + m0, g.ldx, y + row0 * g.ldy + col0, g.ldy,
+                                                     out + (e * g.M + m0) * g.N + col0, g.N, g.M - m0, g.N - col0, terms, g.out, lds);
+    } else {
+        GroupTile t;
+        if (!find_tile<BM, CUT>(g.sizes, blockIdx.x, g.columns, t)) return;
+        int64_t col0 = t.column * BN;
+        if constexpr (CUT) {
+            if (t.parts > 1) {
+                col0 += (t.part & 1) * (BN / 2);
+                t.row0 += (t.part >> 1) * (BM / 2);
+                t.rows -= (t.part >> 1) * (BM / 2);
+                if (t.rows <= 0 || col0 >= g.N) return;
+            }
+        }
+        const bool there = t.group < g.sizes.E;  // else behind the last group: zeros
+        const int64_t terms = there ? g.K : 0;
+        x += t.row0 * g.ldx;
+        y += (there ? t.group : 0) * g.y_group + col0 * (YL == kInner ? g.ldy : 1);
+        out += t.row0 * g.N + col0;
+        if constexpr (CUT) {
+            if (t.parts == 4)
+                return gmm_tile<T, XL, YL, 128, 128, 2, 4, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, t.rows, g.N - col0, terms, g.out, lds);
+            if (t.parts == 2)
+                return gmm_tile<T, XL, YL, 256, 128, 4, 2, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, t.rows, g.N - col0, terms, g.out, lds);
+        }
+        gmm_tile<T, XL, YL, BM, BN, WM, WN, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, t.rows, g.N - col0, terms, g.out, lds);
+    }
 }
 
 }  // namespace trt

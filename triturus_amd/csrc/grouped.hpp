@@ -28,6 +28,7 @@ struct GroupTile {
     int64_t row0;    // first row of the tile
     int64_t rows;    // rows of the group from row0 on (> 0)
     int64_t column;  // column panel
+    int parts, part; // the tile is cut into this many, and this one is meant (find_tile with CUT)
 };
 
 __device__ __forceinline__ int64_t size_at(const Sizes &s, int64_t e) {
@@ -69,7 +70,12 @@ __device__ __forceinline__ void chunk_rows(const Sizes &s, int64_t e, int64_t &b
 // bands of 8 row tiles with the row tile running fastest (neighbours share a panel of the group's matrix),
 // and dealt out to the XCDs in runs of the tiles there ARE: numbering the upper bound instead would
 // leave the last XCDs idle.  Wave-uniform.  The launch has fewer than 2^31 workgroups, so do the tiles.
-template <int BM>
+//
+// CUT: tiles of which a CU holds one at a time run in rounds of kCus, and a last round of a few tiles would take as long as a
+// full one.  Up to kCus / 4 tiles of it are cut into quarters, up to kCus / 2 into halves, which then fill one shorter round
+// (8 groups of 16384 rows in all, K = N = 4096, 1088 tiles of 256 x 256: 560 us in 5 rounds, 520 with quarters).
+constexpr uint32_t kCus = 256;
+template <int BM, bool CUT = false>
 __device__ __forceinline__ bool find_tile(const Sizes &s, uint32_t wg, uint32_t columns, GroupTile &t) {
     const int64_t chunks = s.E / kWave + 1;
     int64_t before = 0, start = 0, end = 0;
@@ -82,10 +88,22 @@ __device__ __forceinline__ bool find_tile(const Sizes &s, uint32_t wg, uint32_t 
         total += n;
     }
     total = __builtin_amdgcn_readfirstlane(total) * columns;
-    const uint32_t per_xcd = (total + kXcds - 1) / kXcds;
-    if (wg >= per_xcd * kXcds) return false;
-    const uint32_t id = (wg % kXcds) * per_xcd + wg / kXcds;
-    if (id >= total) return false;
+    const uint32_t rest = total % kCus;
+    t.parts = !CUT || rest > kCus / 2 ? 1 : rest > kCus / 4 ? 2 : 4;
+    t.part = 0;
+    const uint32_t whole = t.parts > 1 ? total - rest : total, per_xcd = (whole + kXcds - 1) / kXcds;
+    uint32_t id;
+    if (wg < per_xcd * kXcds) {
+        id = (wg % kXcds) * per_xcd + wg / kXcds;
+        if (id >= whole) return false;
+        t.parts = 1;
+    } else {
+        if (t.parts == 1) return false;
+        const uint32_t in = wg - whole;  // the parts of a tile on one XCD
+        id = whole + in / kXcds / t.parts * kXcds + in % kXcds;
+        t.part = in / kXcds % t.parts;
+        if (id >= total) return false;
+    }
     uint32_t first = 0;  // row tiles before the chunk
     before = 0;
     for (int64_t c = 0; c < chunks; ++c) {
@@ -119,6 +137,9 @@ __device__ __forceinline__ void group_rows(const Sizes &s, int64_t e, int64_t &r
     row0 = uniform64(__shfl(start, (int)(e % kWave), kWave));
     rows = uniform64(__shfl(end, (int)(e % kWave), kWave)) - row0;
 }
+
+// Workgroups that find_tile with CUT wants beyond the tiles.
+constexpr int64_t kMostCut = 3 * (kCus / 4) + 4 * kXcds;
 
 inline int64_t most_row_tiles(int64_t T, int64_t E, int BM) { return T / BM + (E + 1 < T ? E + 1 : T); }
 

@@ -1,11 +1,11 @@
 // Products of microscaled 4-bit operands on the scaled matrix pipe: c = a b^T over the values that codes and scales
 // stand for, one matrix for all rows or one per group of rows (sizes on the device).
 //
-// Both operands lie along the contraction, so a 128-byte step of a tile's row is 8 blocks of 32 values, and a lane's 16
+// Both operands lie along the contraction, so a 64-byte step of a tile's row is 4 blocks of 32 values, and a lane's 16
 // bytes of a fragment are one block: v_mfma_scale_f32_32x32x64_f8f6f4 takes them with the block's scale byte and
 // multiplies and scales in one instruction at 4 times the rate of 16-bit operands.  Tiles, staging and LDS
-// layout are those of gmm.hpp (the INNER layout in bytes); the 8 scale bytes of a row's step go with them as
-// one 8-byte word, from which a lane reads the two pairs of its half: blocks 2 kk + (lane >= 32), kk = 0..3.
+// layout are those of gmm.hpp (the INNER layout in bytes); the 4 scale bytes of a row's step go with them as
+// one word, from which a lane reads the two of its half: blocks 2 kk + (lane >= 32), kk = 0, 1.
 #include "few.hpp"
 #include "mx4.hpp"
 
@@ -20,18 +20,6 @@ struct Mx4Args {
     uint32_t columns;
     int dtype;  // of c
 };
-
-__device__ __forceinline__ uintx2 load_scales(const uint8_t *p, int64_t left) {
-    uint64_t v = 0;
-    if (left >= 8) {
-        __builtin_memcpy(&v, p, 8);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 7; ++i)
-            if (i < left) v |= (uint64_t)p[i] << (8 * i);
-    }
-    return __builtin_bit_cast(uintx2, v);
-}
 
 __device__ __forceinline__ uint32_t load_scales4(const uint8_t *p, int64_t left) {
     uint32_t v = 0;
@@ -52,24 +40,25 @@ __device__ __forceinline__ floatx16 mx4_mfma(uintx4 x, uint32_t sx, uintx4 y, ui
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(u, v, c, 4, 4, 2 * PAIR, (int)sx, 2 * PAIR, (int)sy);
 }
 
+template <typename T, int BM, int BN, int WM, int WN>
+struct Mx4Lds {
+    static constexpr int THREADS = 64 * WM * WN;
+    static constexpr int CODES = Operand<uint8_t, kInner, BM, THREADS>::LDS + Operand<uint8_t, kInner, BN, THREADS>::LDS;
+    static constexpr int SCALES = (BM + BN) * 16;  // of four steps
+    static constexpr int OUT = OutTile<T, BM, BN, WM, WN>::LDS;
+    static constexpr int BYTES = kStages * CODES + 2 * SCALES > OUT ? kStages * CODES + 2 * SCALES : OUT;
+};
+
+// One tile: codes x, y and scales sx, sy at its first row and column, `bytes` of codes in a row.
 template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED>
-__global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
+__device__ __forceinline__ void mx4_tile(const Mx4Args &g, const uint8_t *x, const uint8_t *sx, const uint8_t *y, const uint8_t *sy, T *out,
+                                         int64_t rows, int64_t cols, int64_t bytes, char *lds) {
     constexpr int THREADS = 64 * WM * WN, RT = BM / WM / 32, CT = BN / WN / 32;
     using X = Operand<uint8_t, kInner, BM, THREADS>;
     using Y = Operand<uint8_t, kInner, BN, THREADS>;
-    constexpr int CODES = X::LDS + Y::LDS, STAGE = CODES + (BM + BN) * 8, OUT = OutTile<T, BM, BN, WM, WN>::LDS;
-    constexpr int NS = (BM + BN) / THREADS;  // scale words of a thread
-    static_assert((BM + BN) % THREADS == 0 && BM % THREADS == 0 || THREADS == BM + BN, "a thread's scales are of one operand");
-    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE > OUT ? 2 * STAGE : OUT];
-
+    using L = Mx4Lds<T, BM, BN, WM, WN>;
+    constexpr int NS = (BM + BN + THREADS - 1) / THREADS;  // scale words of a thread
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    GroupTile t;
-    if (!find_tile<BM>(g.sizes, blockIdx.x, g.columns, t)) return;
-    const int64_t col0 = t.column * BN, rows = t.rows, cols = g.N - col0;
-    const int64_t e = t.group < g.sizes.E ? t.group : 0;
-    const int64_t bytes = t.group < g.sizes.E ? g.bytes : 0;  // behind the last group: zeros
-    const uint8_t *x = g.a + t.row0 * g.lda, *y = g.b + e * g.b_group + col0 * g.ldb;
-    const uint8_t *sx = g.sa + t.row0 * g.ldsa, *sy = g.sb + e * g.sb_group + col0 * g.ldsb;
 
     floatx16 acc[RT][CT];
 #pragma unroll
@@ -80,73 +69,126 @@ __global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
 
     const int wm = wave / WN, wn = wave % WN, l = lane_id();
-    X xs;
-    Y ys;
-    uintx2 scales[NS];
-    auto load = [&](int64_t s) {
-        const int64_t left = bytes - s * 128;
-        xs.template load<ALIGNED>(x + s * 128, g.lda, rows, left, tid);
-        ys.template load<ALIGNED>(y + s * 128, g.ldb, cols, left, tid);
+    const int64_t steps = ceil_div(bytes, kStepBytes);
+    if (steps > 0) {
+        X xs;
+        Y ys;
+        uintx4 scales[NS];
+        const int64_t blocks = bytes / 16;
+        const uint8_t *sp[NS];  // a row or column that does not exist has the scales of the last one that does, and is not written
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const int r = tid + i * THREADS;
-            const bool of_x = r < BM;
-            const int64_t row = of_x ? r : r - BM;
-            const bool there = row < (of_x ? rows : cols);
-            const uint8_t *p = (of_x ? sx + row * g.ldsa : sy + row * g.ldsb) + s * 8;
-            scales[i] = load_scales(p, there ? left / 16 : 0);
+            const int r = tid + i * THREADS < BM + BN ? tid + i * THREADS : BM + BN - 1;
+            const int64_t row = r < BM ? (r < rows ? r : rows - 1) : (r - BM < cols ? r - BM : cols - 1);
+            sp[i] = r < BM ? sx + row * g.ldsa : sy + row * g.ldsb;
         }
-    };
-    auto store = [&](char *to) {
-        xs.store(to, tid);
-        ys.store(to + X::LDS, tid);
+        char *const ring = lds + kStages * L::CODES;  // scales of four steps, and of the next four
+        auto load_scales = [&](int64_t q) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) *reinterpret_cast<uintx2 *>(to + CODES + (tid + i * THREADS) * 8) = scales[i];
-    };
-    const int64_t steps = ceil_div(bytes, 128);
-    if (steps > 0) {
-        load(0);
-        store(lds);
-        if (steps > 1) load(1);
-        lds_barrier();
-    }
-    for (int64_t s = 0; s < steps; ++s) {
-        const char *xl = lds + (s & 1) * STAGE, *yl = xl + X::LDS, *sl = xl + CODES;
-        char *next = lds + ((s + 1) & 1) * STAGE;
-        uintx2 xe[RT], ye[CT];
-        const int half = 8 * (l >> 5);
+            for (int i = 0; i < NS; ++i) scales[i] = load_chunk(sp[i] + q * 16, blocks - q * 16);
+        };
+        auto store_scales = [&](int64_t q) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const uintx2 v = *reinterpret_cast<const uintx2 *>(sl + ((wm * RT + i) * 32 + (l & 31)) * 8);
-            xe[i] = uintx2{v[0] >> half, v[1] >> half};
-        }
+            for (int i = 0; i < NS; ++i)
+                if (NS * THREADS == BM + BN || tid + i * THREADS < BM + BN)
+                    *reinterpret_cast<uintx4 *>(ring + (q & 1) * L::SCALES + (tid + i * THREADS) * 16) = scales[i];
+        };
+        auto load = [&](int64_t s) {  // behind the last step nothing remains, and nothing is read
+            const int64_t left = bytes - s * kStepBytes;
+            xs.template load<ALIGNED>(x + s * kStepBytes, g.lda, rows, left, tid);
+            ys.template load<ALIGNED>(y + s * kStepBytes, g.ldb, cols, left, tid);
+        };
+        auto store = [&](char *to) {
+            xs.store(to, tid);
+            ys.store(to + X::LDS, tid);
+        };
+        uintx4 xf[2][RT], yf[2][CT];
+        uint32_t xe[2][RT], ye[2][CT];  // of this step and the next one, moved to the lane's half
+        auto fragments = [&](const char *from, int kk) {
 #pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            const uintx2 v = *reinterpret_cast<const uintx2 *>(sl + (BM + (wn * CT + j) * 32 + (l & 31)) * 8);
-            ye[j] = uintx2{v[0] >> half, v[1] >> half};
-        }
+            for (int i = 0; i < RT; ++i) xf[kk][i] = X::fragment(from, (wm * RT + i) * 32, kk);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            uintx4 xf[RT], yf[CT];
-#pragma unroll
-            for (int i = 0; i < RT; ++i) xf[i] = X::fragment(xl, (wm * RT + i) * 32, kk);
-#pragma unroll
-            for (int j = 0; j < CT; ++j) yf[j] = Y::fragment(yl, (wn * CT + j) * 32, kk);
+            for (int j = 0; j < CT; ++j) yf[kk][j] = Y::fragment(from + X::LDS, (wn * CT + j) * 32, kk);
+        };
+        auto exponents = [&](int64_t s, int which) {
+            const char *e = ring + ((s >> 2) & 1) * L::SCALES + (s & 3) * 4;
+            const int half = 8 * (l >> 5);
 #pragma unroll
             for (int i = 0; i < RT; ++i)
+                xe[which][i] = *reinterpret_cast<const uint32_t *>(e + ((wm * RT + i) * 32 + (l & 31)) * 16) >> half;
 #pragma unroll
-                for (int j = 0; j < CT; ++j)
-                    acc[i][j] = kk & 1 ? mx4_mfma<1>(yf[j], ye[j][kk / 2], xf[i], xe[i][kk / 2], acc[i][j])
-                                       : mx4_mfma<0>(yf[j], ye[j][kk / 2], xf[i], xe[i][kk / 2], acc[i][j]);
-            if (kk == 0 && s + 1 < steps) {
-                store(next);
-                if (s + 2 < steps) load(s + 2);
+            for (int j = 0; j < CT; ++j)
+                ye[which][j] = *reinterpret_cast<const uint32_t *>(e + (BM + (wn * CT + j) * 32 + (l & 31)) * 16) >> half;
+        };
+        load(0);
+        load_scales(0);
+        store(lds);
+        store_scales(0);
+        load(1);
+        store(lds + L::CODES);
+        load(2);
+        lds_barrier();
+        fragments(lds, 0);
+        exponents(0, 0);
+        char *now = lds, *next = lds + L::CODES, *after = lds + 2 * L::CODES;
+        static_assert(kSub == 2, "two sub-steps: the scale bytes 0 and 2 of the lane's half");
+        for (int64_t s0 = 0; s0 < steps; s0 += 4) {
+            load_scales(s0 / 4 + 1);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t s = s0 + u;
+                if (s >= steps) break;
+                fragments(now, 1);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<0>(yf[0][j], ye[u & 1][j], xf[0][i], xe[u & 1][i], acc[i][j]);
+                if constexpr (ALIGNED) interleave<0, RT + CT, RT * CT>(std::make_integer_sequence<int, 8>());
+                store(after);  // the step that was read last: everyone is past the barrier behind it
+                if (u == 2) store_scales(s0 / 4 + 1);
+                load(s + 3);
+                fragments(next, 0);
+                exponents(s + 1, ~u & 1);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<1>(yf[1][j], ye[u & 1][j], xf[1][i], xe[u & 1][i], acc[i][j]);
+                if constexpr (ALIGNED) interleave<X::N + Y::N, 2 * (RT + CT), RT * CT>(std::make_integer_sequence<int, 8>());
+                lds_barrier();
+                char *const read = now;
+                now = next, next = after, after = read;
             }
         }
-        lds_barrier();
     }
-    T *out = static_cast<T *>(g.out) + t.row0 * g.N + col0;
     store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, g.N, rows, cols, g.out);
+}
+
+// CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
+template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT>
+__global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
+    static_assert(!CUT || (BM == 256 && BN == 256 && WM == 2 && WN == 4), "the parts below");
+    __shared__ __attribute__((aligned(16))) char lds[Mx4Lds<T, BM, BN, WM, WN>::BYTES];
+    GroupTile t;
+    if (!find_tile<BM, CUT>(g.sizes, blockIdx.x, g.columns, t)) return;
+    int64_t col0 = t.column * BN;
+    if constexpr (CUT) {
+        if (t.parts > 1) {
+            col0 += (t.part & 1) * (BN / 2);
+            t.row0 += (t.part >> 1) * (BM / 2);
+            t.rows -= (t.part >> 1) * (BM / 2);
+            if (t.rows <= 0 || col0 >= g.N) return;
+        }
+    }
+    const int64_t e = t.group < g.sizes.E ? t.group : 0;
+    const int64_t bytes = t.group < g.sizes.E ? g.bytes : 0;  // behind the last group: zeros
+    const uint8_t *x = g.a + t.row0 * g.lda, *y = g.b + e * g.b_group + col0 * g.ldb;
+    const uint8_t *sx = g.sa + t.row0 * g.ldsa, *sy = g.sb + e * g.sb_group + col0 * g.ldsb;
+    T *out = static_cast<T *>(g.out) + t.row0 * g.N + col0;
+    if constexpr (CUT) {
+        if (t.parts == 4) return mx4_tile<T, 128, 128, 2, 4, ALIGNED>(g, x, sx, y, sy, out, t.rows, g.N - col0, bytes, lds);
+        if (t.parts == 2) return mx4_tile<T, 256, 128, 4, 2, ALIGNED>(g, x, sx, y, sy, out, t.rows, g.N - col0, bytes, lds);
+    }
+    mx4_tile<T, BM, BN, WM, WN, ALIGNED>(g, x, sx, y, sy, out, t.rows, g.N - col0, bytes, lds);
 }
 
 // Few rows per group (few.hpp): 16 RT rows x 64 columns, the contraction cut over 8 wavefronts.  A wavefront's unit is
@@ -243,12 +285,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(Mx4Args g) {
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED>
+template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT>
 int launch_mx4_tile(Mx4Args g, hipStream_t s) {
     g.columns = (uint32_t)ceil_div(g.N, BN);
-    const int64_t blocks = ceil_div(most_row_tiles(g.sizes.T, g.sizes.E, BM) * (int64_t)g.columns, kXcds) * kXcds;
+    const int64_t blocks = ceil_div(most_row_tiles(g.sizes.T, g.sizes.E, BM) * (int64_t)g.columns, kXcds) * kXcds + (CUT ? kMostCut : 0);
     if (blocks >= (int64_t)1 << 31) return TRT_E_RANGE;
-    hipLaunchKernelGGL((mx4_mm_kernel<T, BM, BN, WM, WN, ALIGNED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, s, g);
+    hipLaunchKernelGGL((mx4_mm_kernel<T, BM, BN, WM, WN, ALIGNED, CUT>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, s, g);
     return (int)hipGetLastError();
 }
 
@@ -262,18 +304,21 @@ int launch_mx4_few(Mx4Args g, bool aligned, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-// RT of the few-row kernel for this many rows per group on average, 0: 128 x 128 tiles.  tile forces 1 + RT, or 1 for 0.
-inline int few_row_tiles(int64_t T, int64_t E, int tile) {
-    if (tile) return tile - 1;
+// Tiles: 1 = 128 x 128, 2, 3 = 16, 32 rows x 64 columns of the few-row kernel, 4 = 256 x 256.
+inline int choose_mx4_tile(int64_t T, int64_t E, int tile) {
+    if (tile) return tile;
     const int64_t mean = T / E;
-    return mean <= 16 ? 1 : mean <= 32 ? 2 : 0;
+    return mean <= 16 ? 2 : mean <= 32 ? 3 : 1;
 }
 
 template <typename T>
-int launch_mx4(const Mx4Args &g, hipStream_t s) {
+int launch_mx4(const Mx4Args &g, int tile, hipStream_t s) {
     const bool aligned = ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | (uint64_t)g.lda | (uint64_t)g.ldb |
                            (uint64_t)g.b_group) & 15) == 0;
-    return aligned ? launch_mx4_tile<T, 128, 128, 2, 2, true>(g, s) : launch_mx4_tile<T, 128, 128, 2, 2, false>(g, s);
+    if constexpr (sizeof(T) == 2) {
+        if (tile == 4) return aligned ? launch_mx4_tile<T, 256, 256, 2, 4, true, true>(g, s) : launch_mx4_tile<T, 256, 256, 2, 4, false, true>(g, s);
+    }
+    return aligned ? launch_mx4_tile<T, 128, 128, 2, 2, true, false>(g, s) : launch_mx4_tile<T, 128, 128, 2, 2, false, false>(g, s);
 }
 
 }  // namespace trt
@@ -281,7 +326,7 @@ int launch_mx4(const Mx4Args &g, hipStream_t s) {
 using namespace trt;
 
 extern "C" size_t trt_mx4_mm_workspace_bytes(int64_t T, int64_t E, int64_t K, int a_type, int tile) {
-    if (a_type < 0 || T <= 0 || E <= 0 || K <= 0 || few_row_tiles(T, E, tile) == 1) return 0;
+    if (a_type < 0 || T <= 0 || E <= 0 || K <= 0 || choose_mx4_tile(T, E, tile) == 2) return 0;
     return (size_t)(T * ceil_div(K, 32) * 17);
 }
 
@@ -299,8 +344,8 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
     // 256 rows of a tile are addressed with 31-bit byte offsets
     constexpr int64_t kMost = (int64_t)1 << 23;
     if (sa[0] >= kMost || sb[1] >= kMost || N >= kMost || K > 2 * kMost) return TRT_E_RANGE;
-    const int few = few_row_tiles(T, E, tile);
     const size_t need = trt_mx4_mm_workspace_bytes(T, E, K, a_type, tile);
+    tile = choose_mx4_tile(T, E, tile);
     if (need && (!workspace || workspace_bytes < need)) return TRT_E_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return TRT_E_LAYOUT;
     Mx4Args g = {};
@@ -318,9 +363,9 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
         g.a = codes, g.sa = scales, g.lda = g.bytes, g.ldsa = g.bytes / 16;
         a_type = -1;
     }
-    if (few) {
+    if (tile == 2 || tile == 3) {
         const bool aligned = ((reinterpret_cast<uintptr_t>(b) | (uint64_t)g.ldb | (uint64_t)g.b_group) & 15) == 0;
-        if (few == 2) return launch_mx4_few<uint8_t, 2>(g, aligned, s);
+        if (tile == 3) return launch_mx4_few<uint8_t, 2>(g, aligned, s);
         switch (a_type) {
             case TRT_F32: return launch_mx4_few<float, 1>(g, aligned, s);
             case TRT_F16: return launch_mx4_few<_Float16, 1>(g, aligned, s);
@@ -329,8 +374,8 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
         }
     }
     switch (dtype) {
-        case TRT_F32: return launch_mx4<float>(g, s);
-        case TRT_F16: return launch_mx4<_Float16>(g, s);
-        default: return launch_mx4<__bf16>(g, s);
+        case TRT_F32: return launch_mx4<float>(g, tile, s);
+        case TRT_F16: return launch_mx4<_Float16>(g, tile, s);
+        default: return launch_mx4<__bf16>(g, tile, s);
     }
 }
