@@ -318,7 +318,7 @@ int trt_mm_bf16(const float *a, const float *b, float *c, int64_t m, int64_t k, 
  * from any address with the ends of rows read value by value.  A row may be at most 8 MiB long or apart
  * (TRT_E_RANGE).  tile: 0 = choose by shape, 1..TRT_GMM_TILES force a tile (experiments, tests).
  */
-#define TRT_GMM_TILES 5
+#define TRT_GMM_TILES 8
 int trt_gmm(const void *a, const void *b, const void *sizes, void *c, int64_t T, int64_t E, int64_t K,
             int64_t N, int64_t lda, const int64_t sb[3], int dtype, int wide_sizes, int tile, void *stream);
 int trt_gmm_weights(const void *a, const void *g, const void *sizes, void *d, int64_t T, int64_t E, int64_t K,

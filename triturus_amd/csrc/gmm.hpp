@@ -307,11 +307,196 @@ __device__ __forceinline__ void gmm_tile(const T *x, int64_t ldx, const T *y, in
     store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, N, rows, cols, base);
 }
 
+// ---- 256 x 256 tiles of aligned 16-bit operands: memory to LDS without registers between ----------------------------
+typedef __attribute__((address_space(3))) void *lds_ptr;
+
+// One operand's share of a 64-byte step, written by buffer loads that go to LDS: a wavefront's load fills 1 KiB there, lane by
+// lane, so the places are fixed and it is the lanes' sources that are permuted.
+//   INNER  [row][4 chunks], chunk c of row r at c ^ (r / 2 % 4);
+//   OUTER  [contracted][row], the 32 bytes p of contracted value k at p ^ (k % 4): a transposing read's 4 x 32 bytes lie in
+//          different banks.
+template <typename T, int LAYOUT, int B, int WAVES>
+struct Direct {
+    static constexpr int KT = kStepBytes / sizeof(T);
+    static constexpr int ROW = LAYOUT == kInner ? kStepBytes : B * (int)sizeof(T);
+    static constexpr int LDS = B * kStepBytes;
+    static constexpr int N = LDS / 1024 / WAVES;  // loads of a wavefront
+    static_assert(sizeof(T) == 2 && LDS % (1024 * WAVES) == 0, "whole loads for every wavefront");
+
+    uint32_t at[N];  // the lane's byte offset from the step's first value, or beyond the extent where the operand ends
+    int depth[N];    // contracted values before the lane's chunk
+
+    __device__ __forceinline__ Direct(int64_t ld, int64_t out, int wave) {
+        const int l = lane_id();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int place = (wave * N + i) * 1024 + l * 16, row = place / ROW, slot = place % ROW / 16;
+            if constexpr (LAYOUT == kInner) {
+                const int c = slot ^ ((row >> 1) & 3);
+                depth[i] = c * 8;
+                at[i] = row < out ? row * (uint32_t)(ld * sizeof(T)) + c * 16 : 0x80000000u;
+            } else {
+                const int c = slot ^ (2 * (row & 3));
+                depth[i] = row;
+                at[i] = c * 8 < out ? row * (uint32_t)(ld * sizeof(T)) + c * 16 : 0x80000000u;
+            }
+        }
+    }
+
+    // base: where the operand's share of a stage begins.  Addresses are one offset from the stage's array: the compiler tells the
+    // arrays apart, and so does not wait for one stage's loads when it reads another, only through short chains of them.
+    __device__ __forceinline__ void load(const T *p, int64_t left, char *stage, int base, int wave) const {
+        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(p, 0x7fffffff);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(stage + (base + (wave * N + i) * 1024)), 16, depth[i] < left ? at[i] : 0x80000000u, 0, 0, 0);
+    }
+
+    static __device__ __forceinline__ uintx4 fragment(const char *stage, int base, int row, int kk) {
+        const int l = lane_id(), half = l >> 5, m = l & 31;
+        if constexpr (LAYOUT == kInner) {
+            const int r = row + m;
+            return *reinterpret_cast<const uintx4 *>(stage + (base + r * ROW + (((2 * kk + half) ^ ((r >> 1) & 3)) * 16)));
+        } else {
+            typedef short short4v __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) short4v *lds4;
+            const int k = 16 * kk + 8 * half + ((l & 15) >> 2), pair = row / 16 + (m >> 4);
+            const int at = base + k * ROW + ((pair ^ (k & 3)) * 32) + 8 * (l & 3);
+            const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<char *>(stage + at));
+            const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<char *>(stage + (at + 4 * ROW)));
+            const uintx2 a = __builtin_bit_cast(uintx2, lo), b = __builtin_bit_cast(uintx2, hi);
+            return uintx4{a[0], a[1], b[0], b[1]};
+        }
+    }
+};
+
+// Waits until the wavefront's own LDS reads are done and at most LEFT of its loads are on their way, then for the workgroup.  (A
+// release fence would wait for all loads to LDS.)
+template <int LEFT>
+__device__ __forceinline__ void direct_barrier() {
+    static_assert(LEFT < 16, "the low bits of vmcnt");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | LEFT);  // lgkmcnt 0, expcnt any, vmcnt LEFT
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Writes a finished tile of aligned rows, 32 rows of a wavefront at a time through 32 x 32 CT values of LDS; 16-byte chunk c of
+// row r at c ^ (r % PER).  acc as for store_tile.
+template <typename T, int RT, int CT>
+__device__ __forceinline__ void store_direct(const floatx16 (&acc)[RT][CT], char *lds, int wave, int wm, int wn, T *out, int64_t N, int64_t rows,
+                                             int64_t cols) {
+    constexpr int V = 8, PER = CT * 4, STEP = kWave / PER;
+    char *mine = lds + wave * (32 * CT * 32 * (int)sizeof(T));
+    const int l = lane_id();
+    const int64_t wcols = cols - wn * (CT * 32);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int64_t row0 = (wm * RT + i) * 32;
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; q += 4) {
+                struct alignas(8) { T v[4]; } four;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) four.v[u] = (T)acc[i][j][q + u];
+                const int row = l & 31, col = 32 * j + 2 * q + 4 * (l >> 5);
+                *reinterpret_cast<decltype(four) *>(mine + row * (PER * 16) + (((col / V) ^ (row % PER)) * 16) + col % V * 2) = four;
+            }
+        const int c = l % PER;
+#pragma unroll
+        for (int r = l / PER; r < 32; r += STEP) {
+            const uintx4 v = *reinterpret_cast<const uintx4 *>(mine + r * (PER * 16) + ((c ^ (r % PER)) * 16));
+            if (row0 + r < rows && c * V < wcols) *reinterpret_cast<uintx4 *>(out + (row0 + r) * N + wn * (CT * 32) + c * V) = v;
+        }
+    }
+}
+
+template <typename T, int XL, int YL, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T *y, int64_t ldy, T *out, int64_t N, int64_t rows, int64_t cols,
+                                                int64_t terms, char *st0, char *st1, char *st2, char *st3) {
+    constexpr int RT = BM / WM / 32, CT = BN / WN / 32;
+    using X = Direct<T, XL, BM, WM * WN>;
+    using Y = Direct<T, YL, BN, WM * WN>;
+    constexpr int KT = X::KT;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wm = wave / WN, wn = wave % WN;
+    const int64_t x_step = XL == kInner ? KT : KT * ldx, y_step = YL == kInner ? KT : KT * ldy;
+    floatx16 acc[RT][CT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+    const int64_t steps = ceil_div(terms, KT);
+    if (steps > 0) {
+        const X xs(ldx, rows, wave);
+        const Y ys(ldy, cols, wave);
+        auto load = [&](int64_t s, char *to) {
+            const int64_t left = terms - s * KT;
+            xs.load(x + s * x_step, left, to, 0, wave);
+            ys.load(y + s * y_step, left, to, X::LDS, wave);
+        };
+        uintx4 xf[2][RT], yf[2][CT];
+        auto fragments = [&](const char *from, int kk) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) xf[kk][i] = X::fragment(from, 0, (wm * RT + i) * 32, kk);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) yf[kk][j] = Y::fragment(from, X::LDS, (wn * CT + j) * 32, kk);
+        };
+        auto multiply = [&](int kk) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) acc[i][j] = Mfma<T>::step(yf[kk][j], xf[kk][i], acc[i][j]);
+        };
+        constexpr int XR = XL == kInner ? 1 : 2, YR = YL == kInner ? 1 : 2, READS = RT * XR + CT * YR;
+        auto step = [&](int64_t s, const char *now, const char *next, char *fill) {
+            fragments(now, 1);
+            multiply(0);
+            interleave<0, READS, RT * CT>(std::make_integer_sequence<int, 8>());
+            load(s + 3, fill);
+            fragments(next, 0);
+            multiply(1);
+            direct_barrier<X::N + Y::N>();  // the loads of the step after next have landed
+        };
+        load(0, st0);
+        load(1, st1);
+        load(2, st2);
+        direct_barrier<X::N + Y::N>();
+        fragments(st0, 0);
+        for (int64_t s = 0;;) {
+            step(s, st0, st1, st3);
+            if (++s >= steps) break;
+            step(s, st1, st2, st0);
+            if (++s >= steps) break;
+            step(s, st2, st3, st1);
+            if (++s >= steps) break;
+            step(s, st3, st0, st2);
+            if (++s >= steps) break;
+        }
+        direct_barrier<0>();  // nothing is on its way to LDS any more
+    }
+    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, N, rows, cols);
+}
+
 // CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT>
-__global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
+__global__ __launch_bounds__(64 * WM *WN, (BM * BN / (WM * WN) > 4096 && WM * WN == 4) ? 2 : 1) void gmm_kernel(GmmArgs g) {
     static_assert(!CUT || (BM == 256 && BN == 256 && WM == 2 && WN == 4 && XL == kInner), "the parts below");
-    __shared__ __attribute__((aligned(16))) char lds[GmmLds<T, XL, YL, BM, BN, WM, WN>::BYTES];
+    constexpr bool DIRECT = ALIGNED && BM == 256 && sizeof(T) == 2;
+    constexpr int STAGE = DIRECT ? 512 * kStepBytes : 16;
+    __shared__ __attribute__((aligned(1024))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[STAGE];
+    __shared__ __attribute__((aligned(16))) char lds[DIRECT ? 16 : GmmLds<T, XL, YL, BM, BN, WM, WN>::BYTES];
+    auto tile = [&](auto bm, auto bn, auto wm, auto wn, const T *x, const T *y, T *out, int64_t rows, int64_t cols, int64_t terms) {
+        constexpr int M = decltype(bm)::value, N = decltype(bn)::value, P = decltype(wm)::value, Q = decltype(wn)::value;
+        if constexpr (DIRECT) gmm_direct_tile<T, XL, YL, M, N, P, Q>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, st0, st1, st2, st3);
+        else gmm_tile<T, XL, YL, M, N, P, Q, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, g.out, lds);
+    };
+    constexpr std::integral_constant<int, BM> bm;
+    constexpr std::integral_constant<int, BN> bn;
+    constexpr std::integral_constant<int, WM> wm;
+    constexpr std::integral_constant<int, WN> wn;
     const T *x = static_cast<const T *>(g.x), *y = static_cast<const T *>(g.y);
     T *out = static_cast<T *>(g.out);
     if constexpr (XL == kOuter) {
@@ -329,8 +514,7 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
         const int64_t m0 = (int64_t)(band * kBand + in_band % high) * BM, col0 = (int64_t)(in_band / high) * BN;
         int64_t row0, terms;
         group_rows(g.sizes, e, row0, terms);
-        gmm_tile<T, XL, YL, BM, BN, WM, WN, ALIGNED>(x + row0 * g.ldx + m0, g.ldx, y + row0 * g.ldy + col0, g.ldy,
-                                                     out + (e * g.M + m0) * g.N + col0, g.N, g.M - m0, g.N - col0, terms, g.out, lds);
+        tile(bm, bn, wm, wn, x + row0 * g.ldx + m0, y + row0 * g.ldy + col0, out + (e * g.M + m0) * g.N + col0, g.M - m0, g.N - col0, terms);
     } else {
         GroupTile t;
         if (!find_tile<BM, CUT>(g.sizes, blockIdx.x, g.columns, t)) return;
@@ -349,12 +533,13 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
         y += (there ? t.group : 0) * g.y_group + col0 * (YL == kInner ? g.ldy : 1);
         out += t.row0 * g.N + col0;
         if constexpr (CUT) {
-            if (t.parts == 4)
-                return gmm_tile<T, XL, YL, 128, 128, 2, 4, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, t.rows, g.N - col0, terms, g.out, lds);
-            if (t.parts == 2)
-                return gmm_tile<T, XL, YL, 256, 128, 4, 2, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, t.rows, g.N - col0, terms, g.out, lds);
+            constexpr std::integral_constant<int, 128> half;
+            constexpr std::integral_constant<int, 2> two;
+            constexpr std::integral_constant<int, 4> four;
+            if (t.parts == 4) return tile(half, half, two, four, x, y, out, t.rows, g.N - col0, terms);
+            if (t.parts == 2) return tile(bm, half, four, two, x, y, out, t.rows, g.N - col0, terms);
         }
-        gmm_tile<T, XL, YL, BM, BN, WM, WN, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, t.rows, g.N - col0, terms, g.out, lds);
+        tile(bm, bn, wm, wn, x, y, out, t.rows, g.N - col0, terms);
     }
 }
 

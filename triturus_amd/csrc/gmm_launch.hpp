@@ -111,8 +111,8 @@ int launch_gmm(const GmmArgs &g, int64_t E, int64_t T_rows, int tile, hipStream_
                        : launch_gmm_tile<T, XL, YL, 64, 64, 2, 2, false>(g, E, T_rows, s);
     }
     if constexpr (sizeof(T) == 2) {
-        if (tile == 5)
-            return aligned ? launch_gmm_tile<T, XL, YL, 256, 256, 2, 4, true, XL == kInner>(g, E, T_rows, s)
+        if (tile == 5)  // whose aligned form also writes whole chunks
+            return aligned && chunks_aligned<T>(g.out, {g.N}) ? launch_gmm_tile<T, XL, YL, 256, 256, 2, 4, true, XL == kInner>(g, E, T_rows, s)
                            : launch_gmm_tile<T, XL, YL, 256, 256, 2, 4, false, XL == kInner>(g, E, T_rows, s);
     }
     return aligned ? launch_gmm_tile<T, XL, YL, 128, 128, 2, 2, true>(g, E, T_rows, s)

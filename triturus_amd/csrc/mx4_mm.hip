@@ -163,11 +163,113 @@ __device__ __forceinline__ void mx4_tile(const Mx4Args &g, const uint8_t *x, con
     store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, g.N, rows, cols, g.out);
 }
 
+// 256 x 256 tiles (and their parts) of codes at 16-byte boundaries: codes from memory to LDS without registers between
+// (Direct in gmm.hpp, on codes four at a time), scales of four steps as one 16-byte load a row.
+template <typename T, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t *x, const uint8_t *sx, const uint8_t *y, const uint8_t *sy, T *out,
+                                                int64_t rows, int64_t cols, int64_t bytes, char *st0, char *st1, char *st2, char *st3,
+                                                char *ring) {
+    constexpr int RT = BM / WM / 32, CT = BN / WN / 32, SCALES = (BM + BN) * 16;
+    static_assert(BM + BN <= 64 * WM * WN, "a thread has one row's scales");
+    using X = Direct<uint16_t, kInner, BM, WM * WN>;
+    using Y = Direct<uint16_t, kInner, BN, WM * WN>;
+    constexpr int LOADS = X::N + Y::N;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), wm = wave / WN, wn = wave % WN, l = lane_id();
+    floatx16 acc[RT][CT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+    const int64_t steps = ceil_div(bytes, kStepBytes);
+    if (steps > 0) {
+        const X xs(g.lda / 2, rows, wave);
+        const Y ys(g.ldb / 2, cols, wave);
+        auto load = [&](int64_t s, char *to) {
+            const int64_t left = (bytes - s * kStepBytes) / 2;
+            xs.load(reinterpret_cast<const uint16_t *>(x + s * kStepBytes), left, to, 0, wave);
+            ys.load(reinterpret_cast<const uint16_t *>(y + s * kStepBytes), left, to, X::LDS, wave);
+        };
+        const int64_t blocks = bytes / 16;
+        const int r = tid < BM + BN ? tid : BM + BN - 1;
+        // a row or column that does not exist has the scales of the last one that does, and is not written
+        const int64_t row = r < BM ? (r < rows ? r : rows - 1) : (r - BM < cols ? r - BM : cols - 1);
+        const uint8_t *sp = r < BM ? sx + row * g.ldsa : sy + row * g.ldsb;
+        uintx4 scales;
+        auto load_scales = [&](int64_t q) { scales = load_chunk(sp + q * 16, blocks - q * 16); };
+        auto store_scales = [&](int64_t q) {
+            if (BM + BN == 64 * WM * WN || tid < BM + BN) *reinterpret_cast<uintx4 *>(ring + ((q & 1) * SCALES + tid * 16)) = scales;
+        };
+        uintx4 xf[2][RT], yf[2][CT];
+        uint32_t xe[2][RT], ye[2][CT];  // of this step and the next one, moved to the lane's half
+        auto fragments = [&](const char *from, int kk) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) xf[kk][i] = X::fragment(from, 0, (wm * RT + i) * 32, kk);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) yf[kk][j] = Y::fragment(from, X::LDS, (wn * CT + j) * 32, kk);
+        };
+        auto exponents = [&](int64_t s, int which) {
+            const int e = (int)((s >> 2) & 1) * SCALES + (int)(s & 3) * 4, half = 8 * (l >> 5);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                xe[which][i] = *reinterpret_cast<const uint32_t *>(ring + (e + ((wm * RT + i) * 32 + (l & 31)) * 16)) >> half;
+#pragma unroll
+            for (int j = 0; j < CT; ++j)
+                ye[which][j] = *reinterpret_cast<const uint32_t *>(ring + (e + (BM + (wn * CT + j) * 32 + (l & 31)) * 16)) >> half;
+        };
+        static_assert(kSub == 2, "two sub-steps: the scale bytes 0 and 2 of the lane's half");
+        // U: the step's place in its four.  The scales of the next four are asked for in the first and stored in the third.
+        auto step = [&](auto u, int64_t s, const char *now, const char *next, char *fill) {
+            constexpr int U = decltype(u)::value;
+            if constexpr (U == 0) load_scales(s / 4 + 1);
+            fragments(now, 1);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<0>(yf[0][j], ye[U & 1][j], xf[0][i], xe[U & 1][i], acc[i][j]);
+            interleave<0, RT + CT, RT * CT>(std::make_integer_sequence<int, 8>());
+            load(s + 3, fill);
+            if constexpr (U == 2) store_scales(s / 4 + 1);
+            fragments(next, 0);
+            exponents(s + 1, ~U & 1);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<1>(yf[1][j], ye[U & 1][j], xf[1][i], xe[U & 1][i], acc[i][j]);
+            direct_barrier<LOADS>();  // the loads of the step after next have landed
+        };
+        load(0, st0);
+        load_scales(0);
+        store_scales(0);
+        load(1, st1);
+        load(2, st2);
+        direct_barrier<LOADS>();
+        fragments(st0, 0);
+        exponents(0, 0);
+        for (int64_t s = 0;;) {
+            step(std::integral_constant<int, 0>(), s, st0, st1, st3);
+            if (++s >= steps) break;
+            step(std::integral_constant<int, 1>(), s, st1, st2, st0);
+            if (++s >= steps) break;
+            step(std::integral_constant<int, 2>(), s, st2, st3, st1);
+            if (++s >= steps) break;
+            step(std::integral_constant<int, 3>(), s, st3, st0, st2);
+            if (++s >= steps) break;
+        }
+        direct_barrier<0>();  // nothing is on its way to LDS any more
+    }
+    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, g.N, rows, cols);
+}
+
 // CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
-template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT>
+// DIRECT: codes and rows of c at 16-byte boundaries, T of 16 bits.
+template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT, bool DIRECT>
 __global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
     static_assert(!CUT || (BM == 256 && BN == 256 && WM == 2 && WN == 4), "the parts below");
-    __shared__ __attribute__((aligned(16))) char lds[Mx4Lds<T, BM, BN, WM, WN>::BYTES];
+    constexpr int STAGE = DIRECT ? 512 * kStepBytes : 16;
+    __shared__ __attribute__((aligned(1024))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[STAGE], ring[DIRECT ? 2 * 512 * 16 : 16];
+    __shared__ __attribute__((aligned(16))) char lds[DIRECT ? 16 : Mx4Lds<T, BM, BN, WM, WN>::BYTES];
     GroupTile t;
     if (!find_tile<BM, CUT>(g.sizes, blockIdx.x, g.columns, t)) return;
     int64_t col0 = t.column * BN;
@@ -184,11 +286,19 @@ __global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
     const uint8_t *x = g.a + t.row0 * g.lda, *y = g.b + e * g.b_group + col0 * g.ldb;
     const uint8_t *sx = g.sa + t.row0 * g.ldsa, *sy = g.sb + e * g.sb_group + col0 * g.ldsb;
     T *out = static_cast<T *>(g.out) + t.row0 * g.N + col0;
+    auto tile = [&](auto bm, auto bn, auto wm, auto wn) {
+        constexpr int M = decltype(bm)::value, N = decltype(bn)::value, P = decltype(wm)::value, Q = decltype(wn)::value;
+        if constexpr (DIRECT) mx4_direct_tile<T, M, N, P, Q>(g, x, sx, y, sy, out, t.rows, g.N - col0, bytes, st0, st1, st2, st3, ring);
+        else mx4_tile<T, M, N, P, Q, ALIGNED>(g, x, sx, y, sy, out, t.rows, g.N - col0, bytes, lds);
+    };
     if constexpr (CUT) {
-        if (t.parts == 4) return mx4_tile<T, 128, 128, 2, 4, ALIGNED>(g, x, sx, y, sy, out, t.rows, g.N - col0, bytes, lds);
-        if (t.parts == 2) return mx4_tile<T, 256, 128, 4, 2, ALIGNED>(g, x, sx, y, sy, out, t.rows, g.N - col0, bytes, lds);
+        constexpr std::integral_constant<int, 128> half;
+        constexpr std::integral_constant<int, 2> two;
+        constexpr std::integral_constant<int, 4> four;
+        if (t.parts == 4) return tile(half, half, two, four);
+        if (t.parts == 2) return tile(std::integral_constant<int, 256>(), half, four, two);
     }
-    mx4_tile<T, BM, BN, WM, WN, ALIGNED>(g, x, sx, y, sy, out, t.rows, g.N - col0, bytes, lds);
+    tile(std::integral_constant<int, BM>(), std::integral_constant<int, BN>(), std::integral_constant<int, WM>(), std::integral_constant<int, WN>());
 }
 
 // Few rows per group (few.hpp): 16 RT rows x 64 columns, the contraction cut over 8 wavefronts.  A wavefront's unit is
@@ -285,12 +395,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(Mx4Args g) {
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT>
+template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT = false, bool DIRECT = false>
 int launch_mx4_tile(Mx4Args g, hipStream_t s) {
     g.columns = (uint32_t)ceil_div(g.N, BN);
     const int64_t blocks = ceil_div(most_row_tiles(g.sizes.T, g.sizes.E, BM) * (int64_t)g.columns, kXcds) * kXcds + (CUT ? kMostCut : 0);
     if (blocks >= (int64_t)1 << 31) return TRT_E_RANGE;
-    hipLaunchKernelGGL((mx4_mm_kernel<T, BM, BN, WM, WN, ALIGNED, CUT>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, s, g);
+    hipLaunchKernelGGL((mx4_mm_kernel<T, BM, BN, WM, WN, ALIGNED, CUT, DIRECT>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, s, g);
     return (int)hipGetLastError();
 }
 
@@ -316,9 +426,12 @@ int launch_mx4(const Mx4Args &g, int tile, hipStream_t s) {
     const bool aligned = ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | (uint64_t)g.lda | (uint64_t)g.ldb |
                            (uint64_t)g.b_group) & 15) == 0;
     if constexpr (sizeof(T) == 2) {
-        if (tile == 4) return aligned ? launch_mx4_tile<T, 256, 256, 2, 4, true, true>(g, s) : launch_mx4_tile<T, 256, 256, 2, 4, false, true>(g, s);
+        const bool out_aligned = ((reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.N * (int64_t)sizeof(T))) & 15) == 0;
+        if (tile == 4)
+            return aligned && out_aligned ? launch_mx4_tile<T, 256, 256, 2, 4, true, true, true>(g, s)
+                                          : launch_mx4_tile<T, 256, 256, 2, 4, false, true>(g, s);
     }
-    return aligned ? launch_mx4_tile<T, 128, 128, 2, 2, true, false>(g, s) : launch_mx4_tile<T, 128, 128, 2, 2, false, false>(g, s);
+    return aligned ? launch_mx4_tile<T, 128, 128, 2, 2, true>(g, s) : launch_mx4_tile<T, 128, 128, 2, 2, false>(g, s);
 }
 
 }  // namespace trt
