@@ -314,15 +314,22 @@ int trt_mm_bf16(const float *a, const float *b, float *c, int64_t m, int64_t k, 
  * a and b's last two strides exchanged it makes a's gradient.
  * trt_gmm_weights: d[e, k, n] = sum_{r in e} a[r, k] g[r, n], the gradient of b; d: E x K x N, dense; zeros
  * for a group without rows.
- * 16-byte loads of whole chunks where bases and strides allow (all of them multiples of 16 bytes), otherwise chunks
- * from any address with the ends of rows read value by value.  A row may be at most 8 MiB long or apart
- * (TRT_E_RANGE).  tile: 0 = choose by shape, 1..TRT_GMM_TILES force a tile (experiments, tests).
+ * Operands whose base, strides and rows are multiples of 16 bytes are fastest.  Others are read as they lie, or, where that pays,
+ * copied first: that takes a workspace of trt_gmm_workspace_bytes(...) or trt_gmm_weights_workspace_bytes(...) bytes for the
+ * same arguments (usually 0), 16-byte aligned; without it they are read as they lie.  A row may be at most 8 MiB long
+ * or apart, T and E below 2^31 (TRT_E_RANGE).  tile: 0 = choose by shape, 1..TRT_GMM_TILES force a tile (experiments, tests).
  */
-#define TRT_GMM_TILES 8
+#define TRT_GMM_TILES 5
 int trt_gmm(const void *a, const void *b, const void *sizes, void *c, int64_t T, int64_t E, int64_t K,
-            int64_t N, int64_t lda, const int64_t sb[3], int dtype, int wide_sizes, int tile, void *stream);
+            int64_t N, int64_t lda, const int64_t sb[3], int dtype, int wide_sizes, int tile, void *workspace,
+            size_t workspace_bytes, void *stream);
+size_t trt_gmm_workspace_bytes(const void *a, const void *b, int64_t T, int64_t E, int64_t K, int64_t N, int64_t lda,
+                               const int64_t sb[3], int dtype, int tile);
 int trt_gmm_weights(const void *a, const void *g, const void *sizes, void *d, int64_t T, int64_t E, int64_t K,
-                    int64_t N, int64_t lda, int64_t ldg, int dtype, int wide_sizes, int tile, void *stream);
+                    int64_t N, int64_t lda, int64_t ldg, int dtype, int wide_sizes, int tile, void *workspace,
+                    size_t workspace_bytes, void *stream);
+size_t trt_gmm_weights_workspace_bytes(const void *a, const void *g, int64_t T, int64_t E, int64_t K, int64_t N,
+                                       int64_t lda, int64_t ldg, int dtype, int tile);
 
 /*
  * The microscaled 4-bit format (MXFP4 of the OCP Microscaling Formats specification v1.0): blocks of 32 values
@@ -342,7 +349,7 @@ int trt_gmm_weights(const void *a, const void *g, const void *sizes, void *d, in
  * codes may lie at any address (fastest at multiples of 16 bytes) and at most 8 MiB apart (TRT_E_RANGE).
  * a_type: -1 for codes and scales, or TRT_F32, TRT_F16, TRT_BF16 for T x K values that the call quantises
  * itself (sa[0]: row stride in values; a_scales unused), with a workspace of
- * trt_mx4_mm_workspace_bytes(T, E, K, a_type, tile) bytes, 16-byte aligned; 0 where the product's kernel quantises
+ * trt_mx4_mm_workspace_bytes(T, E, K, N, a_type, dtype, tile) bytes, 16-byte aligned; 0 where the product's kernel quantises
  * on the way.  tile: 0 = choose by shape, 1..TRT_MX4_TILES force a tile (experiments, tests).
  */
 #define TRT_MX4_TILES 4
@@ -352,7 +359,7 @@ int trt_mx4_dequantize(const void *codes, const void *scales, void *y, int64_t r
 int trt_mx4_mm(const void *a, const void *a_scales, const void *b, const void *b_scales, const void *sizes, void *c,
                int64_t T, int64_t E, int64_t K, int64_t N, const int64_t sa[2], const int64_t sb[4], int a_type,
                int dtype, int wide_sizes, int tile, void *workspace, size_t workspace_bytes, void *stream);
-size_t trt_mx4_mm_workspace_bytes(int64_t T, int64_t E, int64_t K, int a_type, int tile);
+size_t trt_mx4_mm_workspace_bytes(int64_t T, int64_t E, int64_t K, int64_t N, int a_type, int dtype, int tile);
 
 /*
  * The router of a mixture layer.  logits: T x E (TRT_F32, TRT_F16, TRT_BF16; row stride ld, unit trailing stride).  A row

@@ -225,3 +225,28 @@ def test_every_tile(dev, tile, dtype):
             s = torch.tensor(sizes, device=dev)
             close(_forward(a, b, s, tile), product64(a, b, sizes), product64(a.abs(), b.abs(), sizes), K)
             close(_weights(a, g, s, tile), weights64(a, g, sizes), weights64(a.abs(), g.abs(), sizes), max(sizes))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N", [40, 500, 2000, 6000])
+def test_few_rows_over_many_columns(dev, N, dtype):
+    """One or two rows under the widths at which a tile of few rows changes its columns or wavefronts."""
+    for K in (8, 264, 2056):
+        for layout in ("kn", "nk"):
+            check(*operands(dev, 3, 2, K, N, dtype, layout), [2, 1])
+
+
+def test_many_groups_and_saturating_sizes(dev):
+    """More groups than a wavefront has lanes, with sums of sizes beyond 32 bits."""
+    E, K, N = 200, 16, 24
+    a, b, g = operands(dev, 500, E, K, N, torch.float32)
+    sizes = [(7 * e) % 6 for e in range(E)]
+    sizes[-1] += 500 - sum(sizes) if sum(sizes) < 500 else 0
+    while sum(sizes) > 500:
+        sizes[max(range(E), key=lambda e: sizes[e])] -= 1
+    check(a, b, g, sizes)
+    big = [3] * 150 + [2 ** 31 - 1] * 50
+    s = torch.tensor(big, dtype=torch.int32, device=dev)
+    fit = torch.tensor([3] * 150 + [50] + [0] * 49, dtype=torch.int32, device=dev)
+    assert torch.equal(gmm(a, b, s), gmm(a, b, fit))
+    assert torch.equal(gmm_grad(g, a, b, s.long())[1], gmm_grad(g, a, b, fit)[1])

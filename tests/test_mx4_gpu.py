@@ -263,3 +263,14 @@ def test_every_tile(dev, tile, dtype):
         assert torch.equal(want.isnan(), c.cpu().isnan()) and not want.isnan().all()
         fine = ~want.isnan()
         close(c.cpu()[fine], want[fine], size[fine], K)
+
+
+@pytest.mark.parametrize("N", [40, 500, 3000, 6000])
+def test_few_rows_over_many_columns(dev, N):
+    """One or two rows under the widths at which a tile of few rows changes its columns; values and codes alike."""
+    for K in (32, 128, 160, 2080, 2070):
+        b = mx4_quantize(torch.randn(N, K, device=dev))
+        for dtype in TYPES:
+            a = torch.randn(2, K, device=dev).to(dtype)
+            c = check(a, b)
+            assert torch.equal(mm_mx4(mx4_quantize(a), b, dtype=dtype), c)

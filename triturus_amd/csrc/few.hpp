@@ -1,21 +1,22 @@
 // Products of ragged groups with few rows each (a decoding batch): bound by reading every matrix once.
 //
-// A workgroup makes 16 RT rows x 64 columns of one group, and its 8 wavefronts cut the contraction: no operand is
+// A workgroup makes 16 RT rows x 64 columns of one group, and its W wavefronts cut the contraction: no operand is
 // shared between wavefronts, so the matrix goes from memory straight into MFMA operands (16 x 16 x 32 of 16 bits,
-// 16 x 16 x 4 of fp32) with no barrier before the end, where the 8 partial tiles meet in LDS in a fixed order.
+// 16 x 16 x 4 of fp32) with no barrier before the end, where the W partial tiles meet in LDS in a fixed order.
 // A wavefront's unit is 64 bytes of the contraction by 64 columns:
 //   INNER (contraction contiguous): lane (n, g) reads the 16 bytes g of column n, 4 times for 4 x 16 columns;
 //   OUTER (columns contiguous): lane (c, g) reads, for each of its 16 bytes' worth of contracted values, 4 neighbouring
 //          columns (8 bytes of 16-bit types, 16 of fp32); 16-bit values are turned round in registers, 4 byte
 //          permutations per 4 columns and pair of rows.
-// Two units are in flight per wavefront while a third is multiplied.
+// D units are in flight per wavefront while another is multiplied.  Where 64-column tiles would be fewer than the CUs, an INNER
+// matrix is cut into tiles of 32 or 16 columns with as many more units in flight, an OUTER one among 16 wavefronts.
 #pragma once
 
 #include "gmm.hpp"
 
 namespace trt {
 
-constexpr int kFewWaves = 8, kFewCols = 64;
+constexpr int kFewCols = 64;  // of a workgroup's usual tile
 
 template <typename T>
 struct FewMfma;
@@ -41,56 +42,59 @@ struct FewMfma<float> {
     }
 };
 
-// The 8 wavefronts' parts of a tile, summed in order and written.  acc[i][j][q]: row 16 i + 4 (lane / 16) + q, column
+// LDS of a tile of 16 RT rows and 16 CW columns whose contraction W wavefronts cut.
+template <int RT, int CW, int W>
+struct FewLds {
+    static constexpr int ROW = 16 * CW + 4, PART = 16 * RT * ROW, FLOATS = W * PART;
+};
+
+// The wavefronts' parts of a tile, summed in order and written.  acc[i][j][q]: row 16 i + 4 (lane / 16) + q, column
 // of(j, lane % 16).
-template <typename T, int RT, typename F>
-__device__ __forceinline__ void store_few(const floatx4 (&acc)[RT][4], float *lds, int wave, T *out, int64_t N, int64_t rows, int64_t cols, F of) {
-    constexpr int ROW = kFewCols + 4, PART = 16 * RT * ROW;
+template <typename T, int RT, int CW, int W, typename F>
+__device__ __forceinline__ void store_few(const floatx4 (&acc)[RT][CW], float *lds, int wave, T *out, int64_t N, int64_t rows, int64_t cols, F of) {
+    constexpr int ROW = FewLds<RT, CW, W>::ROW, PART = FewLds<RT, CW, W>::PART, COLS = 16 * CW;
     const int l = lane_id();
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < CW; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) lds[wave * PART + (16 * i + 4 * (l >> 4) + q) * ROW + of(j, l & 15)] = acc[i][j][q];
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * RT * kFewCols; i += 64 * kFewWaves) {
-        const int r = i / kFewCols, c = i % kFewCols;
+    for (int i = threadIdx.x; i < 16 * RT * COLS; i += 64 * W) {
+        const int r = i / COLS, c = i % COLS;
         if (r >= rows || c >= cols) continue;
         float v = lds[r * ROW + c];
 #pragma unroll
-        for (int w = 1; w < kFewWaves; ++w) v += lds[w * PART + r * ROW + c];
+        for (int w = 1; w < W; ++w) v += lds[w * PART + r * ROW + c];
         out[(int64_t)r * N + c] = (T)v;
     }
 }
 
-template <int RT>
-struct FewLds {
-    static constexpr int FLOATS = kFewWaves * 16 * RT * (kFewCols + 4);
-};
-
-template <typename T, int YL, int RT, bool ALIGNED>
-__global__ __launch_bounds__(64 * kFewWaves) void gmm_few_kernel(GmmArgs g) {
+template <typename T, int YL, int RT, bool ALIGNED, int CW = 4, int W = 8, int D = 2>
+__global__ __launch_bounds__(64 * W) void gmm_few_kernel(GmmArgs g) {
+    static_assert(CW == 4 || (YL == kInner && ALIGNED), "4 neighbouring columns of an OUTER matrix are a lane's");
     constexpr int V = 16 / sizeof(T), KT = 64 / sizeof(T);  // values of a chunk, of a unit
+    constexpr int COLS = 16 * CW;
     constexpr int CB = 4 * sizeof(T);                       // bytes of a lane's 4 columns (OUTER)
-    __shared__ float lds[FewLds<RT>::FLOATS];
+    __shared__ float lds[FewLds<RT, CW, W>::FLOATS];
     GroupTile t;
     if (!find_tile<16 * RT>(g.sizes, blockIdx.x, g.columns, t)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = lane_id(), m = l & 15, gk = l >> 4;
-    const int64_t col0 = t.column * kFewCols, rows = t.rows, cols = g.N - col0;
+    const int64_t col0 = t.column * COLS, rows = t.rows, cols = g.N - col0;
     const int64_t terms = t.group < g.sizes.E ? g.K : 0;  // behind the last group: zeros
     const T *x = static_cast<const T *>(g.x) + t.row0 * g.ldx;
     const T *y = static_cast<const T *>(g.y) + (t.group < g.sizes.E ? t.group : 0) * g.y_group + col0 * (YL == kInner ? g.ldy : 1);
 
-    floatx4 acc[RT][4];
+    floatx4 acc[RT][CW];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < CW; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
     struct Unit {
         uintx4 x[RT];
-        uintx4 y[4];  // INNER: 4 columns' chunks; OUTER: V rows of CB bytes
+        uintx4 y[CW];  // INNER: CW columns' chunks; OUTER: V rows of CB bytes
     };
     const int64_t units = ceil_div(terms, KT);
     auto load = [&](int64_t u, Unit &n) {
@@ -105,7 +109,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void gmm_few_kernel(GmmArgs g) {
             }
             if constexpr (YL == kInner) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < CW; ++j) {
                     const int c = 16 * j + m;
                     n.y[j] = __builtin_amdgcn_raw_buffer_load_b128(yr, left > 0 && c < cols ? c * (uint32_t)(g.ldy * sizeof(T)) + gk * 16 : 0x80000000u, 0, 0);
                 }
@@ -175,10 +179,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void gmm_few_kernel(GmmArgs g) {
         }
     };
     auto multiply = [&](const Unit &n) {
-        uintx4 f[4];  // columns' chunks
+        uintx4 f[CW];  // columns' chunks
         if constexpr (YL == kInner) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = n.y[j];
+            for (int j = 0; j < CW; ++j) f[j] = n.y[j];
         } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[j] = uintx4{n.y[0][j], n.y[1][j], n.y[2][j], n.y[3][j]};
@@ -194,20 +198,25 @@ __global__ __launch_bounds__(64 * kFewWaves) void gmm_few_kernel(GmmArgs g) {
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = FewMfma<T>::step(n.x[i], f[j], acc[i][j]);
+            for (int j = 0; j < CW; ++j) acc[i][j] = FewMfma<T>::step(n.x[i], f[j], acc[i][j]);
     };
-    Unit a, b;
-    int64_t u = wave;
-    load(u, a);
-    load(u + kFewWaves, b);
-    for (; u < units; u += 2 * kFewWaves) {
-        multiply(a);
-        load(u + 2 * kFewWaves, a);
-        multiply(b);
-        load(u + 3 * kFewWaves, b);
+    int64_t u = D * wave;  // neighbours: together whole 128-byte lines of an INNER matrix
+    if (u < units) {
+        Unit n[D];
+#pragma unroll
+        for (int d = 0; d < D; ++d) load(u + d, n[d]);
+        for (; u + W * D < units; u += W * D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                multiply(n[d]);
+                load(u + W * D + d, n[d]);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) multiply(n[d]);
     }
-    store_few<T, RT>(acc, lds, wave, static_cast<T *>(g.out) + t.row0 * g.N + col0, g.N, rows, cols,
-                     [](int j, int c) { return YL == kInner ? 16 * j + c : 4 * c + j; });
+    store_few<T, RT, CW, W>(acc, lds, wave, static_cast<T *>(g.out) + t.row0 * g.N + col0, g.N, rows, cols,
+                            [](int j, int c) { return YL == kInner ? 16 * j + c : 4 * c + j; });
 }
 
 }  // namespace trt

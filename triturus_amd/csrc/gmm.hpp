@@ -381,12 +381,13 @@ __device__ __forceinline__ void direct_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// Writes a finished tile of aligned rows, 32 rows of a wavefront at a time through 32 x 32 CT values of LDS; 16-byte chunk c of
+// Writes a finished tile (of 16-bit values), 32 rows of a wavefront at a time through 32 x 32 CT values of LDS; 16-byte chunk c of
 // row r at c ^ (r % PER).  acc as for store_tile.
 template <typename T, int RT, int CT>
 __device__ __forceinline__ void store_direct(const floatx16 (&acc)[RT][CT], char *lds, int wave, int wm, int wn, T *out, int64_t N, int64_t rows,
-                                             int64_t cols) {
+                                             int64_t cols, const void *base) {
     constexpr int V = 8, PER = CT * 4, STEP = kWave / PER;
+    const bool whole = ((reinterpret_cast<uintptr_t>(base) | (uint64_t)(N * (int64_t)sizeof(T))) & 15) == 0;
     char *mine = lds + wave * (32 * CT * 32 * (int)sizeof(T));
     const int l = lane_id();
     const int64_t wcols = cols - wn * (CT * 32);
@@ -407,14 +408,24 @@ __device__ __forceinline__ void store_direct(const floatx16 (&acc)[RT][CT], char
 #pragma unroll
         for (int r = l / PER; r < 32; r += STEP) {
             const uintx4 v = *reinterpret_cast<const uintx4 *>(mine + r * (PER * 16) + ((c ^ (r % PER)) * 16));
-            if (row0 + r < rows && c * V < wcols) *reinterpret_cast<uintx4 *>(out + (row0 + r) * N + wn * (CT * 32) + c * V) = v;
+            if (row0 + r >= rows || c * V >= wcols) continue;
+            T *p = out + (row0 + r) * N + wn * (CT * 32) + c * V;
+            if (whole) {
+                *reinterpret_cast<uintx4 *>(p) = v;
+            } else {
+                T e[V];
+                __builtin_memcpy(e, &v, 16);
+#pragma unroll
+                for (int u = 0; u < V; ++u)
+                    if (c * V + u < wcols) p[u] = e[u];
+            }
         }
     }
 }
 
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN>
 __device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T *y, int64_t ldy, T *out, int64_t N, int64_t rows, int64_t cols,
-                                                int64_t terms, char *st0, char *st1, char *st2, char *st3) {
+                                                int64_t terms, const void *base, char *st0, char *st1, char *st2, char *st3) {
     constexpr int RT = BM / WM / 32, CT = BN / WN / 32;
     using X = Direct<T, XL, BM, WM * WN>;
     using Y = Direct<T, YL, BN, WM * WN>;
@@ -477,7 +488,7 @@ __device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T
         }
         direct_barrier<0>();  // nothing is on its way to LDS any more
     }
-    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, N, rows, cols);
+    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, N, rows, cols, base);
 }
 
 // CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
@@ -490,7 +501,7 @@ __global__ __launch_bounds__(64 * WM *WN, (BM * BN / (WM * WN) > 4096 && WM * WN
     __shared__ __attribute__((aligned(16))) char lds[DIRECT ? 16 : GmmLds<T, XL, YL, BM, BN, WM, WN>::BYTES];
     auto tile = [&](auto bm, auto bn, auto wm, auto wn, const T *x, const T *y, T *out, int64_t rows, int64_t cols, int64_t terms) {
         constexpr int M = decltype(bm)::value, N = decltype(bn)::value, P = decltype(wm)::value, Q = decltype(wn)::value;
-        if constexpr (DIRECT) gmm_direct_tile<T, XL, YL, M, N, P, Q>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, st0, st1, st2, st3);
+        if constexpr (DIRECT) gmm_direct_tile<T, XL, YL, M, N, P, Q>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, g.out, st0, st1, st2, st3);
         else gmm_tile<T, XL, YL, M, N, P, Q, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, g.out, lds);
     };
     constexpr std::integral_constant<int, BM> bm;

@@ -3,8 +3,8 @@
 
 namespace trt {
 
-int gmm_f32(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, hipStream_t s) {
-    return launch_gmm_type<float>(g, E, T_rows, weights, y_inner, tile, s);
+int gmm_f32(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s) {
+    return launch_gmm_type<float>(g, E, T_rows, weights, y_inner, tile, w, s);
 }
 
 }  // namespace trt

@@ -1,11 +1,10 @@
 // The choice of a tile for a product of ragged groups, shared by the element types.
 #pragma once
 
-#include <math.h>
-
 #include <initializer_list>
 
 #include "few.hpp"
+#include "tile_cost.hpp"
 
 namespace trt {
 
@@ -26,13 +25,26 @@ int launch_gmm_tile(GmmArgs g, int64_t E, int64_t T_rows, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-template <typename T, int YL, int RT, bool ALIGNED>
+template <typename T, int YL, int RT, bool ALIGNED, int CW = 4, int W = 8, int D = 2>
 int launch_gmm_few(GmmArgs g, int64_t E, int64_t T_rows, hipStream_t s) {
-    g.columns = (uint32_t)ceil_div(g.N, kFewCols);
+    g.columns = (uint32_t)ceil_div(g.N, 16 * CW);
     const int64_t blocks = ceil_div(most_row_tiles(T_rows, E, 16 * RT) * (int64_t)g.columns, kXcds) * kXcds;
     if (blocks >= (int64_t)1 << 31) return TRT_E_RANGE;
-    hipLaunchKernelGGL((gmm_few_kernel<T, YL, RT, ALIGNED>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, s, g);
+    hipLaunchKernelGGL((gmm_few_kernel<T, YL, RT, ALIGNED, CW, W, D>), dim3((unsigned)blocks), dim3(64 * W), 0, s, g);
     return (int)hipGetLastError();
+}
+
+// 16 rows a tile: more and smaller pieces where there are fewer tiles than CUs.
+template <typename T, int YL>
+int launch_gmm_few_rows(const GmmArgs &g, int64_t E, int64_t T_rows, hipStream_t s) {
+    const double n = GroupedShape(T_rows, E, g.N, 64).tiles(16, kFewCols);
+    if constexpr (YL == kInner) {
+        if (n <= 64) return launch_gmm_few<T, YL, 1, true, 1, 8, 8>(g, E, T_rows, s);
+        if (n <= 128) return launch_gmm_few<T, YL, 1, true, 2, 8, 4>(g, E, T_rows, s);
+    } else if (n <= 256) {
+        return launch_gmm_few<T, YL, 1, true, 4, 16, 2>(g, E, T_rows, s);
+    }
+    return launch_gmm_few<T, YL, 1, true>(g, E, T_rows, s);
 }
 
 template <typename T>
@@ -42,44 +54,27 @@ bool chunks_aligned(const void *p, std::initializer_list<int64_t> values) {
     return (bits & 15) == 0;
 }
 
-// The tile of a rows' product: the least of five estimated times.  The model is fitted to every tile's time on 120 (16-bit) and
-// 50 (fp32) random shapes, 1 to 4096 rows per group; its pick is 2.0 % and 2.6 % behind the best tile timed on average
-// (38 % and 28 % on the worst shape).  `steps` of 64 bytes of the contraction; `tiles` as if groups were equal, with half a
-// tile lost per group.
-//   128 x 128, 256 x 256: microseconds a step with one, two, three workgroups on a CU (256 x 256: a quarter, half or
-//   whole tile on each CU), by rounds;
-//   few rows: a wavefront's chain of units, shared by what a CU holds, or the matrices' bytes at a rate (TB/s).
+// The tile of a rows' product: the least of the estimated times (tile_cost.hpp).
 template <typename T>
-int choose_gmm_tile(int64_t T_rows, int64_t E, int64_t N, int64_t K) {
+int choose_gmm_tile(int64_t T_rows, int64_t E, int64_t N, int64_t K, bool y_inner, double *us = nullptr) {
     constexpr bool F32 = sizeof(T) == 4;
-    const double mean = (double)T_rows / (double)E, groups = (double)(E < T_rows ? E : T_rows);
-    const double steps = (double)ceil_div(K, 64 / (int64_t)sizeof(T));
-    auto tiles = [&](int64_t BM, int64_t BN) {
-        const double high = mean / (double)BM + 0.5;
-        return groups * (high > 1.0 ? high : 1.0) * (double)ceil_div(N, BN);
+    constexpr MidCost kMid = F32 ? MidCost{0.996, 1.90, 2.22, 0.1, 18.6} : MidCost{0.317, 0.440, 1.058, 5.3, 2.0};
+    constexpr BigCost kBig = {0.824, 0.459, 0.276, 3.5, 4.6};
+    constexpr FewCost kFew[2][3] = {{{149, 1.09, 8.0, 5.4}, {147, 1.30, 6.8, 5.9}, {112, 1.80, 5.2, 6.4}},
+                                    {{201, 1.70, 7.6, 3.6}, {172, 2.37, 4.7, 4.4}, {135, 3.64, 8.5, 6.8}}};
+    const GroupedShape g(T_rows, E, N, K * (int64_t)sizeof(T));
+    auto least = [&](double us, double inner, double outer) {  // not below the matrices' reading
+        const double read = g.stream(y_inner ? inner : outer);
+        return us > read ? us : read;
     };
-    auto least = [](double a, double b) { return a < b ? a : b; };
     int best = 1;
-    double best_us;
-    {
-        constexpr double one = F32 ? 0.99 : 0.35, two = F32 ? 2.04 : 0.65, three = F32 ? 3.45 : 1.25, fixed = F32 ? 6.5 : 4.4;
-        const double n = tiles(128, 128), rounds = floor(n / 768), rest = n - 768 * rounds;
-        best_us = fixed + steps * (rounds * three + (rest <= 0 ? 0 : rest <= 256 ? one : rest <= 512 ? two : three));
-    }
+    double best_us = least(estimate(g, kMid), 4.2, 5.4);
     auto consider = [&](int tile, double us) {
         if (us < best_us) best = tile, best_us = us;
     };
-    constexpr double kFew[2][3][4] = {{{141, 1.01, 9.0, 6.0}, {147, 1.35, 7.0, 5.8}, {117, 2.07, 3.66, 5.3}},
-                                      {{201, 1.70, 7.6, 3.6}, {172, 2.37, 4.7, 4.4}, {135, 3.64, 8.5, 6.8}}};
-    for (int i = 0; i < 3; ++i) {
-        const double *k = kFew[F32][i], n = tiles(16 << i, kFewCols);
-        const double chain = ceil(steps / 16) * k[1] * (n > k[0] ? n / k[0] : 1.0), read = n * steps * 4096e-6 / k[2];
-        consider(2 + i, k[3] + (chain > read ? chain : read));
-    }
-    if constexpr (!F32) {
-        const double n = tiles(256, 256), rounds = floor(n / 256), rest = n - 256 * rounds;
-        consider(5, 5.3 + steps * (rounds * 1.30 + least(0.90, rest <= 0 ? 0 : rest <= 64 ? 0.31 : rest <= 128 ? 0.55 : 0.90)));
-    }
+    for (int i = 0; i < 3; ++i) consider(2 + i, least(estimate(g, kFew[F32][i], 1 << i), 4.8, 5.2));
+    if (!F32) consider(5, least(estimate(g, kBig), 4.2, 5.4));
+    if (us) *us = best_us;
     return best;
 }
 
@@ -93,15 +88,109 @@ int choose_weights_tile(int64_t E, int64_t K, int64_t N) {
     return sizeof(T) == 2 && big >= 200 && big * 4 <= mid + mid / 7 ? 5 : 1;
 }
 
+// ---- operands off the 16-byte boundaries -------------------------------------------------------------------------------
+// Rows that start off them, or are not whole chunks, cost every product about twice its time (16-byte loads from any address, and no
+// loads to LDS) and the weights' gradient three times.  Where that is more than a copy, an operand is first copied into
+// rows of whole chunks with zeros behind (16384 rows in 8 groups, K = 2049, N = 2047: 354 us, 210 with both copied; the weights'
+// gradient 508 and 200).
+
+// Rows of n values, `rows` to a group, strides in values, to dense rows of whole chunks.
+struct PadJob {
+    const void *from;
+    void *to;
+    int64_t n, ld, group;
+    Divider chunks, rows;  // of a row, of a group
+    uint32_t total;        // chunks in all
+};
+template <typename T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b, uint32_t a_blocks) {
+    const bool second = blockIdx.x >= a_blocks;
+    const PadJob &j = second ? b : a;
+    const uint32_t i = (blockIdx.x - (second ? a_blocks : 0)) * 256 + threadIdx.x;
+    if (i >= j.total) return;
+    constexpr int V = 16 / sizeof(T);
+    const uint32_t row = divide(i, j.chunks), c = (i - row * j.chunks.d) * V, e = divide(row, j.rows);
+    const T *p = static_cast<const T *>(j.from) + e * j.group + (row - e * j.rows.d) * j.ld + c;
+    static_cast<uintx4 *>(j.to)[i] = load_chunk(p, j.n - c);
+}
+
+struct PadPlan {
+    bool x, y;
+    size_t bytes;  // of workspace
+};
+
+// us: the product's estimated time on aligned operands; worth: how much of it more the others cost.
+template <typename T, int XL, int YL>
+PadPlan plan_pads(const GmmArgs &g, int64_t E, int64_t T_rows, double us, double worth) {
+    constexpr int64_t V = 16 / sizeof(T);
+    const int64_t xn = XL == kInner ? g.K : g.M, yn = YL == kInner ? g.K : g.N, yrows = XL == kOuter ? T_rows : YL == kInner ? E * g.N : E * g.K;
+    PadPlan p = {!chunks_aligned<T>(g.x, {g.ldx, xn}), !chunks_aligned<T>(g.y, {g.ldy, g.y_group, yn}), 0};
+    const int64_t x_chunks = p.x ? T_rows * ceil_div(xn, V) : 0, y_chunks = p.y ? yrows * ceil_div(yn, V) : 0;
+    const double copy = 4.0 + (double)(x_chunks + y_chunks) * 32e-6 / 4.5;
+    if (x_chunks >= (int64_t)1 << 30 || y_chunks >= (int64_t)1 << 30 || copy > worth * us) return {false, false, 0};
+    p.bytes = (size_t)(x_chunks + y_chunks) * 16;
+    return p;
+}
+
+template <typename T, int XL, int YL>
+int apply_pads(GmmArgs &g, int64_t E, int64_t T_rows, const PadPlan &p, void *workspace, hipStream_t s) {
+    if (!p.bytes) return 0;
+    constexpr int64_t V = 16 / sizeof(T);
+    char *to = static_cast<char *>(workspace);
+    auto job = [&](bool wanted, const void *&from, int64_t &ld, int64_t &group, int64_t n, int64_t rows, int64_t groups) {
+        PadJob j = {};
+        if (!wanted) return j;
+        const int64_t chunks = ceil_div(n, V);
+        j = {from, to, n, ld, group, divider((uint32_t)chunks), divider((uint32_t)rows), (uint32_t)(groups * rows * chunks)};
+        from = to;
+        to += (size_t)j.total * 16;
+        ld = chunks * V;
+        group = rows * ld;
+        return j;
+    };
+    int64_t none = 0;
+    const bool matrices = XL == kInner;
+    const PadJob a = job(p.x, g.x, g.ldx, none, XL == kInner ? g.K : g.M, T_rows, 1);
+    const PadJob b = job(p.y, g.y, g.ldy, matrices ? g.y_group : none, YL == kInner ? g.K : g.N, !matrices ? T_rows : YL == kInner ? g.N : g.K,
+                         matrices ? E : 1);
+    const uint32_t a_blocks = (uint32_t)ceil_div(a.total, 256), b_blocks = (uint32_t)ceil_div(b.total, 256);
+    hipLaunchKernelGGL(pad_rows_kernel<T>, dim3(a_blocks + b_blocks), dim3(256), 0, s, a, b, a_blocks);
+    return (int)hipGetLastError();
+}
+
+struct Workspace {
+    void *p;
+    size_t bytes;
+    size_t *query;  // not null: only say how many are wanted
+};
+
 // x: the rows' operand (a; a transposed for the weights), y: the matrices or g.
 template <typename T, int XL, int YL>
-int launch_gmm(const GmmArgs &g, int64_t E, int64_t T_rows, int tile, hipStream_t s) {
-    const bool aligned = chunks_aligned<T>(g.x, {g.ldx, XL == kInner ? g.K : g.M}) &&
-                         chunks_aligned<T>(g.y, {g.ldy, g.y_group, YL == kInner ? g.K : g.N});
-    if (tile == 0) tile = XL == kOuter ? choose_weights_tile<T>(E, g.M, g.N) : choose_gmm_tile<T>(T_rows, E, g.N, g.K);
+int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &w, hipStream_t s) {
+    double us = 0.0;
+    if constexpr (XL == kOuter) {
+        if (tile == 0) tile = choose_weights_tile<T>(E, g.M, g.N);
+        us = 10.0 + 2.0 * (double)T_rows * (double)g.M * (double)g.N / (sizeof(T) == 4 ? 60e6 : 900e6);
+    } else {
+        const int best = choose_gmm_tile<T>(T_rows, E, g.N, g.K, YL == kInner, &us);
+        if (tile == 0) tile = best;
+    }
+    // few rows are bound by reading the matrices, and a copy reads and writes them
+    const bool few = XL == kInner && tile >= 2 && tile <= 4;
+    const PadPlan pads = few ? PadPlan{false, false, 0} : plan_pads<T, XL, YL>(g, E, T_rows, us, XL == kOuter ? 1.2 : 0.8);
+    if (w.query) {
+        *w.query = pads.bytes;
+        return TRT_OK;
+    }
+    bool aligned = chunks_aligned<T>(g.x, {g.ldx, XL == kInner ? g.K : g.M}) && chunks_aligned<T>(g.y, {g.ldy, g.y_group, YL == kInner ? g.K : g.N});
+    if (pads.bytes && w.p && w.bytes >= pads.bytes) {  // without a workspace the operands are read as they are
+        const int status = apply_pads<T, XL, YL>(g, E, T_rows, pads, w.p, s);
+        if (status) return status;
+        aligned = true;
+    }
     if constexpr (XL == kInner) {
         switch (tile) {
-            case 2: return aligned ? launch_gmm_few<T, YL, 1, true>(g, E, T_rows, s) : launch_gmm_few<T, YL, 1, false>(g, E, T_rows, s);
+            case 2: return aligned ? launch_gmm_few_rows<T, YL>(g, E, T_rows, s) : launch_gmm_few<T, YL, 1, false>(g, E, T_rows, s);
             case 3: return aligned ? launch_gmm_few<T, YL, 2, true>(g, E, T_rows, s) : launch_gmm_few<T, YL, 2, false>(g, E, T_rows, s);
             case 4: return aligned ? launch_gmm_few<T, YL, 4, true>(g, E, T_rows, s) : launch_gmm_few<T, YL, 4, false>(g, E, T_rows, s);
             default: break;
@@ -111,8 +200,8 @@ int launch_gmm(const GmmArgs &g, int64_t E, int64_t T_rows, int tile, hipStream_
                        : launch_gmm_tile<T, XL, YL, 64, 64, 2, 2, false>(g, E, T_rows, s);
     }
     if constexpr (sizeof(T) == 2) {
-        if (tile == 5)  // whose aligned form also writes whole chunks
-            return aligned && chunks_aligned<T>(g.out, {g.N}) ? launch_gmm_tile<T, XL, YL, 256, 256, 2, 4, true, XL == kInner>(g, E, T_rows, s)
+        if (tile == 5)
+            return aligned ? launch_gmm_tile<T, XL, YL, 256, 256, 2, 4, true, XL == kInner>(g, E, T_rows, s)
                            : launch_gmm_tile<T, XL, YL, 256, 256, 2, 4, false, XL == kInner>(g, E, T_rows, s);
     }
     return aligned ? launch_gmm_tile<T, XL, YL, 128, 128, 2, 2, true>(g, E, T_rows, s)
@@ -120,13 +209,13 @@ int launch_gmm(const GmmArgs &g, int64_t E, int64_t T_rows, int tile, hipStream_
 }
 
 template <typename T>
-int launch_gmm_type(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, hipStream_t s) {
-    if (weights) return launch_gmm<T, kOuter, kOuter>(g, E, T_rows, tile, s);
-    return y_inner ? launch_gmm<T, kInner, kInner>(g, E, T_rows, tile, s) : launch_gmm<T, kInner, kOuter>(g, E, T_rows, tile, s);
+int launch_gmm_type(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s) {
+    if (weights) return launch_gmm<T, kOuter, kOuter>(g, E, T_rows, tile, w, s);
+    return y_inner ? launch_gmm<T, kInner, kInner>(g, E, T_rows, tile, w, s) : launch_gmm<T, kInner, kOuter>(g, E, T_rows, tile, w, s);
 }
 
-int gmm_bf16(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, hipStream_t s);
-int gmm_f16(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, hipStream_t s);
-int gmm_f32(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, hipStream_t s);
+int gmm_bf16(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s);
+int gmm_f16(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s);
+int gmm_f32(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s);
 
 }  // namespace trt

@@ -4,7 +4,7 @@
 // T rows are cut into E consecutive groups of sizes[e] rows; rows behind the last group are the
 // "tail".  The host knows T and E only, so it launches the most tiles that any sizes can make,
 // T / BM + min(E + 1, T) of them per column panel, and every wavefront finds its own tile by a prefix sum
-// over the sizes (E = 64: one load and six lane steps).  Sizes that do not fit (negative, or past T in
+// over the sizes (one load and a few vector instructions for 64 groups).  Sizes that do not fit (negative, or past T in
 // sum) are clamped there, so no sizes make a kernel leave the tensors.
 #pragma once
 
@@ -31,39 +31,42 @@ struct GroupTile {
     int parts, part; // the tile is cut into this many, and this one is meant (find_tile with CUT)
 };
 
-__device__ __forceinline__ int64_t size_at(const Sizes &s, int64_t e) {
+// T < 2^31 (checked by the host), so rows are 32-bit numbers; sums of clamped sizes saturate.
+__device__ __forceinline__ uint32_t size_at(const Sizes &s, uint32_t e) {
+    const uint32_t T = (uint32_t)s.T;
     if (e >= s.E) return 0;
-    if (!s.p) return s.T;
+    if (!s.p) return T;
     const int64_t v = s.wide ? static_cast<const int64_t *>(s.p)[e] : (int64_t)static_cast<const int32_t *>(s.p)[e];
-    return v < 0 ? 0 : (v > s.T ? s.T : v);
+    return v < 0 ? 0 : (v > (int64_t)T ? T : (uint32_t)v);
 }
 
-__device__ __forceinline__ int64_t wave_prefix(int64_t v) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const int64_t u = __shfl_up(v, d, kWave);
-        if (lane_id() >= d) v += u;
-    }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t v) {
+    return __builtin_amdgcn_update_dpp(0u, v, CTRL, ROWS, 0xf, false);
+}
+// Inclusive prefix sum over the wavefront, six vector instructions deep (moves within rows of 16, then of whole rows).
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+    v = __builtin_elementwise_add_sat(v, dpp_or_zero<0x111, 0xf>(v));  // row_shr 1, 2, 4, 8
+    v = __builtin_elementwise_add_sat(v, dpp_or_zero<0x112, 0xf>(v));
+    v = __builtin_elementwise_add_sat(v, dpp_or_zero<0x114, 0xf>(v));
+    v = __builtin_elementwise_add_sat(v, dpp_or_zero<0x118, 0xf>(v));
+    v = __builtin_elementwise_add_sat(v, dpp_or_zero<0x142, 0xa>(v));  // row_bcast 15: into rows 1 and 3
+    v = __builtin_elementwise_add_sat(v, dpp_or_zero<0x143, 0xc>(v));  // row_bcast 31: into rows 2 and 3
     return v;
 }
-
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
-    return (int64_t)(((uint64_t)hi << 32) | lo);
-}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 // Rows [start, end) of group e + lane, for a chunk of 64 groups from e on; `before` is the sum of the
 // sizes before the chunk and moves on.  Index E is the tail.
-__device__ __forceinline__ void chunk_rows(const Sizes &s, int64_t e, int64_t &before, int64_t &start, int64_t &end) {
-    const int64_t g = e + lane_id();
-    const int64_t incl = before + wave_prefix(size_at(s, g));
-    end = incl < s.T ? incl : s.T;
-    start = __shfl_up(end, 1, kWave);
-    if (lane_id() == 0) start = before < s.T ? before : s.T;
-    if (g == s.E) end = s.T;
-    if (g > s.E) start = end = s.T;
-    before = uniform64(__shfl(incl, kWave - 1, kWave));
+__device__ __forceinline__ void chunk_rows(const Sizes &s, uint32_t e, uint32_t &before, uint32_t &start, uint32_t &end) {
+    const uint32_t g = e + lane_id(), T = (uint32_t)s.T;
+    const uint32_t incl = __builtin_elementwise_add_sat(before, wave_prefix(size_at(s, g)));
+    const uint32_t first = before < T ? before : T;
+    end = incl < T ? incl : T;
+    start = __builtin_amdgcn_update_dpp(first, end, 0x138, 0xf, 0xf, false);  // wave_shr 1; lane 0 keeps `first`
+    if (g == s.E) end = T;
+    if (g > s.E) start = end = T;
+    before = lane_value(incl, kWave - 1);
 }
 
 // The tile of workgroup `wg`, or false when there is none for it.  Tiles are numbered group by group, in
@@ -77,17 +80,14 @@ __device__ __forceinline__ void chunk_rows(const Sizes &s, int64_t e, int64_t &b
 constexpr uint32_t kCus = 256;
 template <int BM, bool CUT = false>
 __device__ __forceinline__ bool find_tile(const Sizes &s, uint32_t wg, uint32_t columns, GroupTile &t) {
-    const int64_t chunks = s.E / kWave + 1;
-    int64_t before = 0, start = 0, end = 0;
-    uint32_t total = 0;
-    for (int64_t c = 0; c < chunks; ++c) {
+    const uint32_t chunks = (uint32_t)s.E / kWave + 1;
+    uint32_t before = 0, start = 0, end = 0, total = 0, incl = 0;
+    for (uint32_t c = 0; c < chunks; ++c) {
         chunk_rows(s, c * kWave, before, start, end);
-        uint32_t n = (uint32_t)ceil_div(end - start, BM);
-#pragma unroll
-        for (int d = kWave / 2; d; d /= 2) n += __shfl_xor(n, d, kWave);
-        total += n;
+        incl = wave_prefix((end - start + (BM - 1)) / BM);
+        total += lane_value(incl, kWave - 1);
     }
-    total = __builtin_amdgcn_readfirstlane(total) * columns;
+    total *= columns;
     const uint32_t rest = total % kCus;
     t.parts = !CUT || rest > kCus / 2 ? 1 : rest > kCus / 4 ? 2 : 4;
     t.part = 0;
@@ -106,42 +106,55 @@ __device__ __forceinline__ bool find_tile(const Sizes &s, uint32_t wg, uint32_t 
     }
     uint32_t first = 0;  // row tiles before the chunk
     before = 0;
-    for (int64_t c = 0; c < chunks; ++c) {
-        if (chunks > 1) chunk_rows(s, c * kWave, before, start, end);
-        const uint32_t n = (uint32_t)ceil_div(end - start, BM);
-        const uint32_t incl = (uint32_t)wave_prefix(n);
+    for (uint32_t c = 0; c < chunks; ++c) {
+        if (chunks > 1) {
+            chunk_rows(s, c * kWave, before, start, end);
+            incl = wave_prefix((end - start + (BM - 1)) / BM);
+        }
         const uint64_t past = __ballot((first + incl) * columns > id);
         if (past) {
             const int who = __builtin_ctzll(past);
-            const uint32_t tiles = __builtin_amdgcn_readfirstlane(__shfl(n, who, kWave));
-            const uint32_t at = id - (first + __builtin_amdgcn_readfirstlane(__shfl(incl, who, kWave)) - tiles) * columns;
+            const uint32_t start_row = lane_value(start, who), end_row = lane_value(end, who);
+            const uint32_t tiles = (end_row - start_row + (BM - 1)) / BM;
+            const uint32_t at = id - (first + lane_value(incl, who) - tiles) * columns;
             constexpr uint32_t kBand = 8;
             const uint32_t band = at / (kBand * columns);
             const uint32_t high = tiles - band * kBand < kBand ? tiles - band * kBand : kBand;
             const uint32_t in = at - band * kBand * columns;
             t.group = c * kWave + who;
-            t.row0 = uniform64(__shfl(start, who, kWave)) + (int64_t)(band * kBand + in % high) * BM;
-            t.rows = uniform64(__shfl(end, who, kWave)) - t.row0;
+            t.row0 = start_row + (band * kBand + in % high) * BM;
+            t.rows = end_row - t.row0;
             t.column = in / high;
             return true;
         }
-        first += __builtin_amdgcn_readfirstlane(__shfl(incl, kWave - 1, kWave));
+        first += lane_value(incl, kWave - 1);
     }
     return false;
 }
 
 // Rows [row0, row0 + rows) of one group.
-__device__ __forceinline__ void group_rows(const Sizes &s, int64_t e, int64_t &row0, int64_t &rows) {
-    int64_t before = 0, start = 0, end = 0;
-    for (int64_t c = 0; c <= e / kWave; ++c) chunk_rows(s, c * kWave, before, start, end);
-    row0 = uniform64(__shfl(start, (int)(e % kWave), kWave));
-    rows = uniform64(__shfl(end, (int)(e % kWave), kWave)) - row0;
+__device__ __forceinline__ void group_rows(const Sizes &s, uint32_t e, int64_t &row0, int64_t &rows) {
+    uint32_t before = 0, start = 0, end = 0;
+    for (uint32_t c = 0; c <= e / kWave; ++c) chunk_rows(s, c * kWave, before, start, end);
+    row0 = lane_value(start, e % kWave);
+    rows = lane_value(end, e % kWave) - row0;
 }
 
 // Workgroups that find_tile with CUT wants beyond the tiles.
 constexpr int64_t kMostCut = 3 * (kCus / 4) + 4 * kXcds;
 
 inline int64_t most_row_tiles(int64_t T, int64_t E, int BM) { return T / BM + (E + 1 < T ? E + 1 : T); }
+
+// n / d for n < 2^31 by one multiplication (d fixed by the host).
+struct Divider {
+    uint32_t d, m, s;
+};
+inline Divider divider(uint32_t d) {
+    uint32_t s = 0;
+    while (((uint64_t)1 << s) < d) ++s;
+    return {d, (uint32_t)(((((uint64_t)1 << s) - d) << 32) / d + 1), s};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divider &v) { return (__umulhi(n, v.m) + n) >> v.s; }
 
 // ---- 16 bytes of a row -----------------------------------------------------------------------------
 // `left` elements of the row remain from p on (<= 0: none).  A full chunk is one load, whatever the

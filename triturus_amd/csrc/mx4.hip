@@ -12,17 +12,6 @@
 
 namespace trt {
 
-// n / d for n < 2^31 by one multiplication (d fixed by the host).
-struct Divider {
-    uint32_t d, m, s;
-};
-inline Divider divider(uint32_t d) {
-    uint32_t s = 0;
-    while (((uint64_t)1 << s) < d) ++s;
-    return {d, (uint32_t)(((((uint64_t)1 << s) - d) << 32) / d + 1), s};
-}
-__device__ __forceinline__ uint32_t divide(uint32_t n, const Divider &v) { return (__umulhi(n, v.m) + n) >> v.s; }
-
 constexpr int kPart = 8;                // values of a lane
 constexpr int kParts = 32 / kPart;      // lanes of a block
 
@@ -40,7 +29,9 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T *__restrict__
     top = max_u(top, __builtin_amdgcn_mov_dpp(top, 0xB1, 0xf, 0xf, true));  // lanes 1 0 3 2 of each four
     top = max_u(top, __builtin_amdgcn_mov_dpp(top, 0x4E, 0xf, 0xf, true));  // lanes 2 3 0 1
     const uint32_t scale = block_scale(top);
-    codes[i] = codes_of(v, scale);
+    uint32_t word[1];
+    codes_of(v, scale, word);
+    codes[i] = word[0];
     if (i % kParts == 0) scales[i / kParts] = (uint8_t)scale;
 }
 

@@ -47,29 +47,35 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t codes, const T *v, float 
     }
 }
 
-// 8 codes under a block's scale.  The conversion divides by a power of two that has to be a normal number, and takes no
+// 8 codes a word under a block's scale.  The conversion divides by a power of two that has to be a normal number, and takes no
 // subnormal values: blocks below 2^-92 (never fp16's) are moved up by 2^32 before, exactly.
-template <typename T>
-__device__ __forceinline__ uint32_t codes_of(const T *v, uint32_t scale) {
-    uint32_t codes = 0;
-    if (scale == 255) return 0;
+template <typename T, int N>
+__device__ __forceinline__ void codes_of(const T (&v)[N], uint32_t scale, uint32_t (&codes)[N / 8]) {
+#pragma unroll
+    for (int w = 0; w < N / 8; ++w) codes[w] = 0;
+    if (scale == 255) return;
     if (scale >= 32 || __is_same(T, _Float16)) {
         const float by = __builtin_bit_cast(float, (scale ? scale : 127) << 23);  // 0: all values are 0
-        codes = code_pair<T, 0>(codes, v, by);
-        codes = code_pair<T, 1>(codes, v + 2, by);
-        codes = code_pair<T, 2>(codes, v + 4, by);
-        codes = code_pair<T, 3>(codes, v + 6, by);
+#pragma unroll
+        for (int w = 0; w < N / 8; ++w) {
+            codes[w] = code_pair<T, 0>(codes[w], v + 8 * w, by);
+            codes[w] = code_pair<T, 1>(codes[w], v + 8 * w + 2, by);
+            codes[w] = code_pair<T, 2>(codes[w], v + 8 * w + 4, by);
+            codes[w] = code_pair<T, 3>(codes[w], v + 8 * w + 6, by);
+        }
     } else {
         const float by = __builtin_bit_cast(float, (scale + 32) << 23);
-        float u[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = (float)v[i] * 0x1p32f;
-        codes = code_pair<float, 0>(codes, u, by);
-        codes = code_pair<float, 1>(codes, u + 2, by);
-        codes = code_pair<float, 2>(codes, u + 4, by);
-        codes = code_pair<float, 3>(codes, u + 6, by);
+        for (int w = 0; w < N / 8; ++w) {
+            float u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = (float)v[8 * w + i] * 0x1p32f;
+            codes[w] = code_pair<float, 0>(codes[w], u, by);
+            codes[w] = code_pair<float, 1>(codes[w], u + 2, by);
+            codes[w] = code_pair<float, 2>(codes[w], u + 4, by);
+            codes[w] = code_pair<float, 3>(codes[w], u + 6, by);
+        }
     }
-    return codes;
 }
 
 // N values from p on, of which `left` exist (<= 0: none); the others are 0.

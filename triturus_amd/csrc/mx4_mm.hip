@@ -8,6 +8,7 @@
 // one word, from which a lane reads the two of its half: blocks 2 kk + (lane >= 32), kk = 0, 1.
 #include "few.hpp"
 #include "mx4.hpp"
+#include "tile_cost.hpp"
 
 namespace trt {
 
@@ -259,11 +260,11 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
         }
         direct_barrier<0>();  // nothing is on its way to LDS any more
     }
-    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, g.N, rows, cols);
+    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, g.N, rows, cols, g.out);
 }
 
 // CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
-// DIRECT: codes and rows of c at 16-byte boundaries, T of 16 bits.
+// DIRECT: codes at 16-byte boundaries, T of 16 bits.
 template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT, bool DIRECT>
 __global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
     static_assert(!CUT || (BM == 256 && BN == 256 && WM == 2 && WN == 4), "the parts below");
@@ -305,93 +306,123 @@ __global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
 // 64 bytes of codes (4 blocks) by 64 columns: lane (n, g) takes block g of columns n, n + 16, .. and a column's 4 scale
 // bytes as one word.  A: the type of a's values, which the lane quantises itself on the way (32 neighbours of a
 // row: no other lane is needed, and a call is one launch), or uint8_t for codes.
-template <typename A, int RT, bool ALIGNED>
-__global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(Mx4Args g) {
-    __shared__ float lds[FewLds<RT>::FLOATS];
+// FAST: at least 4 blocks in a row, and whole ones of values.
+template <typename A, int RT, bool FAST, int CW = 4, int W = 8, int D = 2>
+__global__ __launch_bounds__(64 * W) void mx4_few_kernel(Mx4Args g) {
+    constexpr int COLS = 16 * CW;
+    __shared__ float lds[FewLds<RT, CW, W>::FLOATS];
     GroupTile t;
     if (!find_tile<16 * RT>(g.sizes, blockIdx.x, g.columns, t)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = lane_id(), m = l & 15, gk = l >> 4;
-    const int64_t col0 = t.column * kFewCols, rows = t.rows, cols = g.N - col0;
+    const int64_t col0 = t.column * COLS, rows = t.rows, cols = g.N - col0;
     const int64_t e = t.group < g.sizes.E ? t.group : 0;
     const int64_t bytes = t.group < g.sizes.E ? g.bytes : 0;  // behind the last group: zeros
     const A *x = reinterpret_cast<const A *>(g.a) + t.row0 * g.lda;
     const uint8_t *sx = g.sa + t.row0 * g.ldsa, *y = g.b + e * g.b_group + col0 * g.ldb, *sy = g.sb + e * g.sb_group + col0 * g.ldsb;
 
-    floatx4 acc[RT][4];
+    floatx4 acc[RT][CW];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < CW; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
     constexpr bool VALUES = sizeof(A) != 1;
+    static_assert(FAST || !VALUES, "values are quantised where all blocks are whole");
     struct Unit {
         A x[RT][VALUES ? 32 : 16];
         uint32_t sx[RT];
-        uintx4 y[4];
-        uint32_t sy[4];
+        uintx4 y[CW];
+        uint32_t sy[CW];
+        int64_t u;
     };
     auto load = [&](int64_t u, Unit &n) {
-        const int64_t left = bytes - u * 64 - gk * 16, blocks = bytes / 16 - u * 4;
+        n.u = u;
+        if constexpr (FAST) {
+            // No branch: a row or column that does not exist is read as the last one that does (and not written), a block
+            // behind the last one as the last, under scales made 0: 36 2^-254 at most, which is 0 in fp32.
+            const int64_t word = u * 4 < bytes / 16 - 4 ? u * 4 : bytes / 16 - 4, at = u * 64 + gk * 16;
+            const int rlast = rows < 16 * RT ? (int)rows - 1 : 16 * RT - 1, clast = cols < COLS ? (int)cols - 1 : COLS - 1;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const int r = 16 * i + m;
-            const bool there = r < rows;
-            if constexpr (VALUES) {
-                const int64_t k = u * 128 + gk * 32;
-                load_values(x + r * g.lda + k, there && left > 0 ? g.K - k : 0, n.x[i]);
-            } else {
-                load_values(x + r * g.lda + u * 64 + gk * 16, there ? left : 0, n.x[i]);
-                n.sx[i] = load_scales4(sx + r * g.ldsa + u * 4, there ? blocks : 0);
+            for (int i = 0; i < RT; ++i) {
+                const int r = 16 * i + m < rlast ? 16 * i + m : rlast;
+                if constexpr (VALUES) {
+                    const int64_t k = u * 128 + gk * 32;
+                    __builtin_memcpy(n.x[i], x + r * g.lda + (k < g.K - 32 ? k : g.K - 32), sizeof(n.x[i]));
+                } else {
+                    __builtin_memcpy(n.x[i], reinterpret_cast<const uint8_t *>(x) + r * g.lda + (at < bytes - 16 ? at : bytes - 16), 16);
+                    __builtin_memcpy(&n.sx[i], sx + r * g.ldsa + word, 4);
+                }
             }
-        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = 16 * j + m;
-            if constexpr (ALIGNED) {
-                const __amdgpu_buffer_rsrc_t r = make_rsrc(y + u * 64, 0x7fffffff);
-                n.y[j] = __builtin_amdgcn_raw_buffer_load_b128(r, left > 0 && c < cols ? c * (uint32_t)g.ldb + gk * 16 : 0x80000000u, 0, 0);
-            } else {
+            for (int j = 0; j < CW; ++j) {
+                const int c = 16 * j + m < clast ? 16 * j + m : clast;
+                __builtin_memcpy(&n.y[j], y + c * g.ldb + (at < bytes - 16 ? at : bytes - 16), 16);
+                __builtin_memcpy(&n.sy[j], sy + c * g.ldsb + word, 4);
+            }
+        } else {
+            const int64_t left = bytes - u * 64 - gk * 16, blocks = bytes / 16 - u * 4;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const int r = 16 * i + m;
+                load_values(x + r * g.lda + u * 64 + gk * 16, r < rows ? left : 0, n.x[i]);
+                n.sx[i] = load_scales4(sx + r * g.ldsa + u * 4, r < rows ? blocks : 0);
+            }
+#pragma unroll
+            for (int j = 0; j < CW; ++j) {
+                const int c = 16 * j + m;
                 n.y[j] = load_chunk(y + c * g.ldb + u * 64 + gk * 16, c < cols ? left : 0);
+                n.sy[j] = load_scales4(sy + c * g.ldsb + u * 4, c < cols ? blocks : 0);
             }
-            n.sy[j] = load_scales4(sy + c * g.ldsb + u * 4, c < cols ? blocks : 0);
         }
     };
     auto multiply = [&](const Unit &n) {
         typedef int intx8 __attribute__((ext_vector_type(8)));
         auto wide = [](uintx4 v) { return intx8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
+        // words read before their place, where the row has ended, are moved down to it
+        const int64_t past = FAST && n.u * 4 > bytes / 16 - 4 ? n.u * 4 - (bytes / 16 - 4) : 0;
+        const uint32_t down = (uint32_t)(8 * past) & 31, keep = past < 4 ? ~0u : 0u;
+        auto scale = [&](uint32_t word) { return ((word >> down) & keep) >> (8 * gk); };
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             uintx4 xf;
             uint32_t s;
             if constexpr (VALUES) {
                 s = block_scale(top_bits(n.x[i]));
-                xf = uintx4{codes_of(n.x[i], s), codes_of(n.x[i] + 8, s), codes_of(n.x[i] + 16, s), codes_of(n.x[i] + 24, s)};
+                uint32_t word[4];
+                codes_of(n.x[i], s, word);
+                xf = uintx4{word[0], word[1], word[2], word[3]};
+                s = n.u * 64 + gk * 16 < bytes ? s : 0;
             } else {
-                s = n.sx[i] >> (8 * gk);
+                s = scale(n.sx[i]);
                 __builtin_memcpy(&xf, n.x[i], 16);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(xf), wide(n.y[j]), acc[i][j], 4, 4, 0, (int)s, 0,
-                                                                             (int)(n.sy[j] >> (8 * gk)));
+            for (int j = 0; j < CW; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(xf), wide(n.y[j]), acc[i][j], 4, 4, 0, (int)s, 0, (int)scale(n.sy[j]));
         }
     };
     const int64_t units = ceil_div(bytes, 64);
-    Unit a, b;
-    int64_t u = wave;
-    load(u, a);
-    for (; u < units; u += 2 * kFewWaves) {
-        load(u + kFewWaves, b);
-        multiply(a);
-        load(u + 2 * kFewWaves, a);
-        multiply(b);
+    int64_t u = D * wave;  // neighbours: together whole 128-byte lines of the codes
+    if (u < units) {
+        Unit n[D];
+#pragma unroll
+        for (int d = 0; d < D; ++d) load(u + d, n[d]);
+        for (; u + W * D < units; u += W * D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                multiply(n[d]);
+                load(u + W * D + d, n[d]);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) multiply(n[d]);
     }
     const auto of = [](int j, int c) { return 16 * j + c; };
     const int64_t at = t.row0 * g.N + col0;
     switch (g.dtype) {
-        case TRT_F32: store_few<float, RT>(acc, lds, wave, static_cast<float *>(g.out) + at, g.N, rows, cols, of); break;
-        case TRT_F16: store_few<_Float16, RT>(acc, lds, wave, static_cast<_Float16 *>(g.out) + at, g.N, rows, cols, of); break;
-        default: store_few<__bf16, RT>(acc, lds, wave, static_cast<__bf16 *>(g.out) + at, g.N, rows, cols, of); break;
+        case TRT_F32: store_few<float, RT, CW, W>(acc, lds, wave, static_cast<float *>(g.out) + at, g.N, rows, cols, of); break;
+        case TRT_F16: store_few<_Float16, RT, CW, W>(acc, lds, wave, static_cast<_Float16 *>(g.out) + at, g.N, rows, cols, of); break;
+        default: store_few<__bf16, RT, CW, W>(acc, lds, wave, static_cast<__bf16 *>(g.out) + at, g.N, rows, cols, of); break;
     }
 }
 
@@ -404,21 +435,47 @@ int launch_mx4_tile(Mx4Args g, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-template <typename A, int RT>
-int launch_mx4_few(Mx4Args g, bool aligned, hipStream_t s) {
-    g.columns = (uint32_t)ceil_div(g.N, kFewCols);
+template <typename A, int RT, bool FAST, int CW = 4, int W = 8, int D = 2>
+int launch_mx4_few(Mx4Args g, hipStream_t s) {
+    g.columns = (uint32_t)ceil_div(g.N, 16 * CW);
     const int64_t blocks = ceil_div(most_row_tiles(g.sizes.T, g.sizes.E, 16 * RT) * (int64_t)g.columns, kXcds) * kXcds;
     if (blocks >= (int64_t)1 << 31) return TRT_E_RANGE;
-    if (aligned) hipLaunchKernelGGL((mx4_few_kernel<A, RT, true>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, s, g);
-    else hipLaunchKernelGGL((mx4_few_kernel<A, RT, false>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, s, g);
+    hipLaunchKernelGGL((mx4_few_kernel<A, RT, FAST, CW, W, D>), dim3((unsigned)blocks), dim3(64 * W), 0, s, g);
     return (int)hipGetLastError();
 }
 
-// Tiles: 1 = 128 x 128, 2, 3 = 16, 32 rows x 64 columns of the few-row kernel, 4 = 256 x 256.
-inline int choose_mx4_tile(int64_t T, int64_t E, int tile) {
+// 16 rows a tile: more and smaller pieces where there are fewer tiles than CUs.
+template <typename A>
+int launch_mx4_few_rows(const Mx4Args &g, hipStream_t s) {
+    const double n = GroupedShape(g.sizes.T, g.sizes.E, g.N, 64).tiles(16, kFewCols);
+    if (n <= 64) return launch_mx4_few<A, 1, true, 1, 8, 4>(g, s);
+    if (n <= 128) return launch_mx4_few<A, 1, true, 2, 8, 4>(g, s);
+    return launch_mx4_few<A, 1, true>(g, s);
+}
+
+// Tiles: 1 = 128 x 128, 2, 3 = 16, 32 rows x 64 columns of the few-row kernel, 4 = 256 x 256 (c of 16-bit types); the least of
+// the estimated times (tile_cost.hpp).
+inline int choose_mx4_tile(int64_t T, int64_t E, int64_t K, int64_t N, int dtype, int tile) {
     if (tile) return tile;
-    const int64_t mean = T / E;
-    return mean <= 16 ? 2 : mean <= 32 ? 3 : 1;
+    constexpr MidCost kMid = {0.410, 0.740, 1.634, 4.7, 7.4};
+    constexpr BigCost kBig = {0.897, 0.795, 0.445, 3.3, 7.7};
+    constexpr FewCost kFew[2] = {{107, 1.10, 4.5, 6.3}, {127, 2.81, 2.7, 5.5}};
+    const GroupedShape g(T, E, N, ceil_div(K, 32) * 16);
+    int best = 1;
+    double best_us = estimate(g, kMid);
+    auto consider = [&](int t, double us) {
+        if (us < best_us) best = t, best_us = us;
+    };
+    for (int i = 0; i < 2; ++i) consider(2 + i, estimate(g, kFew[i], 1 << i));
+    if (dtype != TRT_F32) consider(4, estimate(g, kBig));
+    return best;
+}
+
+// The few-row kernel quantises a's values itself where its workgroups are few: each makes the codes of its rows again, which costs
+// less than a launch up to about a round of workgroups (2 rows, one matrix of 3392 x 4672: 15.0 us a call, 12.4 from
+// codes; 8 groups of 6 rows, 7328 x 416: 32 and 17, and the launch takes 2.3).
+inline bool quantizes_on_the_way(int64_t T, int64_t E, int64_t K, int64_t N, int tile) {
+    return tile == 2 && K % 32 == 0 && K >= 128 && GroupedShape(T, E, N, 64).tiles(16, kFewCols) <= 300;
 }
 
 template <typename T>
@@ -426,10 +483,9 @@ int launch_mx4(const Mx4Args &g, int tile, hipStream_t s) {
     const bool aligned = ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | (uint64_t)g.lda | (uint64_t)g.ldb |
                            (uint64_t)g.b_group) & 15) == 0;
     if constexpr (sizeof(T) == 2) {
-        const bool out_aligned = ((reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.N * (int64_t)sizeof(T))) & 15) == 0;
         if (tile == 4)
-            return aligned && out_aligned ? launch_mx4_tile<T, 256, 256, 2, 4, true, true, true>(g, s)
-                                          : launch_mx4_tile<T, 256, 256, 2, 4, false, true>(g, s);
+            return aligned ? launch_mx4_tile<T, 256, 256, 2, 4, true, true, true>(g, s)
+                           : launch_mx4_tile<T, 256, 256, 2, 4, false, true>(g, s);
     }
     return aligned ? launch_mx4_tile<T, 128, 128, 2, 2, true>(g, s) : launch_mx4_tile<T, 128, 128, 2, 2, false>(g, s);
 }
@@ -438,8 +494,9 @@ int launch_mx4(const Mx4Args &g, int tile, hipStream_t s) {
 
 using namespace trt;
 
-extern "C" size_t trt_mx4_mm_workspace_bytes(int64_t T, int64_t E, int64_t K, int a_type, int tile) {
-    if (a_type < 0 || T <= 0 || E <= 0 || K <= 0 || choose_mx4_tile(T, E, tile) == 2) return 0;
+extern "C" size_t trt_mx4_mm_workspace_bytes(int64_t T, int64_t E, int64_t K, int64_t N, int a_type, int dtype, int tile) {
+    if (a_type < 0 || T <= 0 || E <= 0 || K <= 0 || N <= 0) return 0;
+    if (quantizes_on_the_way(T, E, K, N, choose_mx4_tile(T, E, K, N, dtype, tile))) return 0;
     return (size_t)(T * ceil_div(K, 32) * 17);
 }
 
@@ -456,9 +513,9 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
         if (sb[i] < 0) return TRT_E_LAYOUT;
     // 256 rows of a tile are addressed with 31-bit byte offsets
     constexpr int64_t kMost = (int64_t)1 << 23;
-    if (sa[0] >= kMost || sb[1] >= kMost || N >= kMost || K > 2 * kMost) return TRT_E_RANGE;
-    const size_t need = trt_mx4_mm_workspace_bytes(T, E, K, a_type, tile);
-    tile = choose_mx4_tile(T, E, tile);
+    if (sa[0] >= kMost || sb[1] >= kMost || N >= kMost || K > 2 * kMost || T >= (int64_t)1 << 31 || E >= (int64_t)1 << 31) return TRT_E_RANGE;
+    const size_t need = trt_mx4_mm_workspace_bytes(T, E, K, N, a_type, dtype, tile);
+    tile = choose_mx4_tile(T, E, K, N, dtype, tile);
     if (need && (!workspace || workspace_bytes < need)) return TRT_E_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return TRT_E_LAYOUT;
     Mx4Args g = {};
@@ -477,13 +534,13 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
         a_type = -1;
     }
     if (tile == 2 || tile == 3) {
-        const bool aligned = ((reinterpret_cast<uintptr_t>(b) | (uint64_t)g.ldb | (uint64_t)g.b_group) & 15) == 0;
-        if (tile == 3) return launch_mx4_few<uint8_t, 2>(g, aligned, s);
+        const bool fast = g.bytes >= 64;
+        if (tile == 3) return fast ? launch_mx4_few<uint8_t, 2, true>(g, s) : launch_mx4_few<uint8_t, 2, false>(g, s);
         switch (a_type) {
-            case TRT_F32: return launch_mx4_few<float, 1>(g, aligned, s);
-            case TRT_F16: return launch_mx4_few<_Float16, 1>(g, aligned, s);
-            case TRT_BF16: return launch_mx4_few<__bf16, 1>(g, aligned, s);
-            default: return launch_mx4_few<uint8_t, 1>(g, aligned, s);
+            case TRT_F32: return launch_mx4_few_rows<float>(g, s);
+            case TRT_F16: return launch_mx4_few_rows<_Float16>(g, s);
+            case TRT_BF16: return launch_mx4_few_rows<__bf16>(g, s);
+            default: return fast ? launch_mx4_few_rows<uint8_t>(g, s) : launch_mx4_few<uint8_t, 1, false>(g, s);
         }
     }
     switch (dtype) {

@@ -88,23 +88,19 @@ __device__ __forceinline__ void set_bit(uint64_t *mask, int row) {
 }
 
 // First place of every expert, over all workgroups: `first` holds the counts and becomes their exclusive prefix sum;
-// returns the sum.  256 threads, `part` has a slot per wavefront.
+// returns the sum.  `part` has a slot per wavefront.
+template <int THREADS>
 __device__ __forceinline__ uint32_t prefix_experts(uint32_t *first, int E, uint32_t *part) {
     uint32_t before = 0;
     const int tid = threadIdx.x, w = tid / kWave;
-    for (int e0 = 0; e0 < E; e0 += 256) {
+    for (int e0 = 0; e0 < E; e0 += THREADS) {
         const int e = e0 + tid;
-        const uint32_t n = e < E ? first[e] : 0;
-        uint32_t incl = n;
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const uint32_t u = __shfl_up(incl, d, kWave);
-            if (lane_id() >= d) incl += u;
-        }
+        const uint32_t n = e < E ? first[e] : 0, incl = wave_prefix(n);
         if (lane_id() == kWave - 1) part[w] = incl;
         __syncthreads();
         uint32_t add = before, all = 0;
-        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int i = 0; i < THREADS / kWave; ++i) {
             if (i < w) add += part[i];
             all += part[i];
         }
@@ -116,10 +112,11 @@ __device__ __forceinline__ uint32_t prefix_experts(uint32_t *first, int E, uint3
 }
 
 // Writes the pairs of the workgroup's rows: `first[e]` is the place of the expert's first pair in this workgroup.
+template <int THREADS>
 __device__ __forceinline__ void place_pairs(const RouteArgs &g, int64_t row0, const uint64_t *mask, const uint32_t *first,
                                             const int32_t *chosen, uint32_t total) {
     const int64_t rows = g.T - row0 < kRouteRows ? g.T - row0 : kRouteRows;
-    for (int i = threadIdx.x; i < rows * g.k; i += 256) {
+    for (int i = threadIdx.x; i < rows * g.k; i += THREADS) {
         const int32_t e = chosen[i];
         const int row = i / g.k;
         int32_t slot = -1;
@@ -133,16 +130,22 @@ __device__ __forceinline__ void place_pairs(const RouteArgs &g, int64_t row0, co
 }
 
 // V * 16 >= E.  ONE: a single workgroup, which also orders the pairs.
+// 16 wavefronts take all 64 rows at once (a choice is a chain of dependent steps); 4 where a lane's 64 logits leave no
+// registers for more.
+template <int V>
+constexpr int kChooseThreads = V > 32 ? 256 : 1024;
+
 template <typename T, int V, bool ONE>
-__global__ __launch_bounds__(256) void route_choose_kernel(RouteArgs g) {
+__global__ __launch_bounds__(kChooseThreads<V>) void route_choose_kernel(RouteArgs g) {
+    constexpr int THREADS = kChooseThreads<V>;
     __shared__ uint64_t mask[V * 16];
     __shared__ int32_t chosen[ONE ? kRouteRows * kRouteMost : 1];
-    __shared__ uint32_t first[ONE ? V * 16 : 1], part[4];
-    for (int e = threadIdx.x; e < g.E; e += 256) mask[e] = 0;
+    __shared__ uint32_t first[ONE ? V * 16 : 1], part[THREADS / kWave];
+    for (int e = threadIdx.x; e < g.E; e += THREADS) mask[e] = 0;
     __syncthreads();
     const int lane = threadIdx.x & 15, shift = lane_id() & 48;
     const int64_t row0 = (int64_t)blockIdx.x * kRouteRows;
-    for (int r = threadIdx.x / 16; r < kRouteRows; r += 16) {
+    for (int r = threadIdx.x / 16; r < kRouteRows; r += THREADS / 16) {
         const int64_t t = row0 + r;
         if (t >= g.T) break;  // whole rows of 16 lanes
         float x[V];
@@ -189,7 +192,7 @@ __global__ __launch_bounds__(256) void route_choose_kernel(RouteArgs g) {
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < g.E; e += 256) {
+    for (int e = threadIdx.x; e < g.E; e += THREADS) {
         const uint32_t n = __builtin_popcountll(mask[e]);
         if constexpr (ONE) {
             g.sizes[e] = (int32_t)n;
@@ -200,8 +203,8 @@ __global__ __launch_bounds__(256) void route_choose_kernel(RouteArgs g) {
     }
     if constexpr (ONE) {
         __syncthreads();
-        const uint32_t total = prefix_experts(first, g.E, part);
-        place_pairs(g, row0, mask, first, chosen, total);
+        const uint32_t total = prefix_experts<THREADS>(first, g.E, part);
+        place_pairs<THREADS>(g, row0, mask, first, chosen, total);
     }
 }
 
@@ -215,12 +218,7 @@ __global__ __launch_bounds__(256) void route_prefix_kernel(RouteArgs g, int64_t 
     for (int64_t b0 = 0; b0 < workgroups; b0 += 256) {
         const int64_t b = b0 + threadIdx.x;
         const uint32_t n = b < workgroups ? counts[b] : 0;
-        uint32_t incl = n;
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const uint32_t u = __shfl_up(incl, d, kWave);
-            if (lane_id() >= d) incl += u;
-        }
+        const uint32_t incl = wave_prefix(n);
         if (lane_id() == kWave - 1) part[w] = incl;
         __syncthreads();
         uint32_t add = before, all = 0;
@@ -266,10 +264,10 @@ __global__ __launch_bounds__(256) void route_place_kernel(RouteArgs g, int64_t w
         const int32_t e = chosen[i];
         if (e >= 0) set_bit(&mask[e], i / g.k);
     }
-    const uint32_t total = prefix_experts(first, g.E, part);
+    const uint32_t total = prefix_experts<256>(first, g.E, part);
     for (int e = threadIdx.x; e < g.E; e += 256) first[e] += before[e];
     __syncthreads();
-    place_pairs(g, row0, mask, first, chosen, total);
+    place_pairs<256>(g, row0, mask, first, chosen, total);
 }
 
 struct RouteGradArgs {
@@ -342,8 +340,8 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
 
 template <typename T, int V>
 void launch_choose(const RouteArgs &g, int64_t workgroups, hipStream_t s) {
-    if (workgroups == 1) hipLaunchKernelGGL((route_choose_kernel<T, V, true>), dim3(1), dim3(256), 0, s, g);
-    else hipLaunchKernelGGL((route_choose_kernel<T, V, false>), dim3((unsigned)workgroups), dim3(256), 0, s, g);
+    if (workgroups == 1) hipLaunchKernelGGL((route_choose_kernel<T, V, true>), dim3(1), dim3(kChooseThreads<V>), 0, s, g);
+    else hipLaunchKernelGGL((route_choose_kernel<T, V, false>), dim3((unsigned)workgroups), dim3(kChooseThreads<V>), 0, s, g);
 }
 
 template <typename T>

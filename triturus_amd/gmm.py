@@ -84,11 +84,17 @@ def _forward(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor, tile: int = 
     if K == 0:
         return c.zero_()
     a, b, sizes = _rows(a), _matrices(b), sizes.contiguous()
+    lib, code = _lib.load(), _lib.DTYPE_CODES[dtype]
+    pa, pb, lda, sb = a.data_ptr(), b.data_ptr(), a.stride(0), _lib.strides3(b)
+    ws_ptr, nbytes, ws = None, 0, None
+    if (pa | pb) & 15 or (K | N | lda | sb[0] | (sb[2] if sb[1] == 1 else sb[1])) & 7:  # then a copy may pay
+        nbytes = lib.trt_gmm_workspace_bytes(pa, pb, T, E, K, N, lda, sb, code, tile)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws_ptr = ws.data_ptr()
     with _lib.on_device(dev):
-        status = _lib.load().trt_gmm(
-            a.data_ptr(), b.data_ptr(), sizes.data_ptr(), c.data_ptr(), T, E, K, N, a.stride(0), _lib.strides3(b),
-            _lib.DTYPE_CODES[dtype], sizes.dtype is torch.int64, tile, _lib.raw_stream(dev),
-        )
+        status = lib.trt_gmm(pa, pb, sizes.data_ptr(), c.data_ptr(), T, E, K, N, lda, sb, code, sizes.dtype is torch.int64, tile,
+                             ws_ptr, nbytes, _lib.raw_stream(dev))
     if status:
         _lib.check(status, "trt_gmm")
     return c
@@ -104,11 +110,17 @@ def _weights(a: torch.Tensor, g: torch.Tensor, sizes: torch.Tensor, tile: int = 
     if T == 0:
         return d.zero_()
     a, g, sizes = _rows(a), _rows(g), sizes.contiguous()
+    lib, code = _lib.load(), _lib.DTYPE_CODES[dtype]
+    pa, pg, lda, ldg = a.data_ptr(), g.data_ptr(), a.stride(0), g.stride(0)
+    ws_ptr, nbytes, ws = None, 0, None
+    if (pa | pg) & 15 or (K | N | lda | ldg) & 7:  # then a copy may pay
+        nbytes = lib.trt_gmm_weights_workspace_bytes(pa, pg, T, E, K, N, lda, ldg, code, tile)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws_ptr = ws.data_ptr()
     with _lib.on_device(dev):
-        status = _lib.load().trt_gmm_weights(
-            a.data_ptr(), g.data_ptr(), sizes.data_ptr(), d.data_ptr(), T, E, K, N, a.stride(0), g.stride(0),
-            _lib.DTYPE_CODES[dtype], sizes.dtype is torch.int64, tile, _lib.raw_stream(dev),
-        )
+        status = lib.trt_gmm_weights(pa, pg, sizes.data_ptr(), d.data_ptr(), T, E, K, N, lda, ldg, code, sizes.dtype is torch.int64, tile,
+                                     ws_ptr, nbytes, _lib.raw_stream(dev))
     if status:
         _lib.check(status, "trt_gmm_weights")
     return d

@@ -112,7 +112,7 @@ def mx4_dequantize(q: MX4, *, dtype: torch.dtype = torch.float32) -> torch.Tenso
     return y
 
 
-_ws_bytes: dict = {}  # (T, E, K, type of a) -> workspace bytes, as reported by the library
+_ws_bytes: dict = {}  # (T, E, K, N, types, tile) -> workspace bytes, as reported by the library
 
 
 def mm_mx4(a: torch.Tensor | MX4, b: MX4, sizes: torch.Tensor | None = None, *, dtype: torch.dtype | None = None,
@@ -161,7 +161,7 @@ def mm_mx4(a: torch.Tensor | MX4, b: MX4, sizes: torch.Tensor | None = None, *, 
     lib = _lib.load()
     nbytes = 0
     if a_type >= 0:
-        key = (T, E, K, a_type, _tile)
+        key = (T, E, K, N, a_type, code, _tile)
         nbytes = _ws_bytes.get(key)
         if nbytes is None:
             if len(_ws_bytes) > 4096:
