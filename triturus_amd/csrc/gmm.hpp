@@ -516,7 +516,7 @@ __global__ __launch_bounds__(64 * WM *WN, (BM * BN / (WM * WN) > 4096 && WM * WN
         // group to group, so that matrices of few tiles fill all XCDs too.  (8 groups of 2048 rows on average, K = N = 4096: 1390 us
         // with a group per XCD, 680 us so.)
         const uint32_t per = g.row_tiles * g.columns, run = (per + kXcds - 1) / kXcds;
-        const uint32_t e = blockIdx.x / kXcds / run;
+        uint32_t e = blockIdx.x / kXcds / run;
         const uint32_t in = (blockIdx.x + e) % kXcds * run + blockIdx.x / kXcds % run;
         if (in >= per) return;
         constexpr uint32_t kBand = 8;
@@ -524,7 +524,8 @@ __global__ __launch_bounds__(64 * WM *WN, (BM * BN / (WM * WN) > 4096 && WM * WN
         const uint32_t high = g.row_tiles - band * kBand < kBand ? g.row_tiles - band * kBand : kBand;
         const int64_t m0 = (int64_t)(band * kBand + in_band % high) * BM, col0 = (int64_t)(in_band / high) * BN;
         int64_t row0, terms;
-        group_rows(g.sizes, e, row0, terms);
+        if (g.sizes.E <= kWave) e = group_by_length(g.sizes, e, row0, terms);  // long ones first: the last round is made of short ones
+        else group_rows(g.sizes, e, row0, terms);
         tile(bm, bn, wm, wn, x + row0 * g.ldx + m0, y + row0 * g.ldy + col0, out + (e * g.M + m0) * g.N + col0, g.M - m0, g.N - col0, terms);
     } else {
         GroupTile t;

@@ -9,7 +9,7 @@
 namespace trt {
 
 // Tiles of the rows' products: 1 = 128 x 128, 2, 3, 4 = 16, 32, 64 rows x 64 columns of the few-row kernel, 5 = 256 x 256
-// (16-bit types).  Of the weights' gradient: 1 = 128 x 128, 2 = 64 x 64, 5 = 256 x 256.
+// (16-bit types) or 64 x 64 (fp32).  Of the weights' gradient: 1 = 128 x 128, 2 = 64 x 64, 5 = 256 x 256.
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT = false>
 int launch_gmm_tile(GmmArgs g, int64_t E, int64_t T_rows, hipStream_t s) {
     g.columns = (uint32_t)ceil_div(g.N, BN);
@@ -58,10 +58,11 @@ bool chunks_aligned(const void *p, std::initializer_list<int64_t> values) {
 template <typename T>
 int choose_gmm_tile(int64_t T_rows, int64_t E, int64_t N, int64_t K, bool y_inner, double *us = nullptr) {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr MidCost kMid = F32 ? MidCost{0.996, 1.90, 2.22, 0.1, 18.6} : MidCost{0.317, 0.440, 1.058, 5.3, 2.0};
+    constexpr MidCost kMid = F32 ? MidCost{0.980, 1.98, 2.91, 2.4, 11.4} : MidCost{0.317, 0.440, 1.058, 5.3, 2.0};
     constexpr BigCost kBig = {0.824, 0.459, 0.276, 3.5, 4.6};
+    constexpr SmallCost kSmall = {0.340, 0.293, 4.5};  // fp32
     constexpr FewCost kFew[2][3] = {{{149, 1.09, 8.0, 5.4}, {147, 1.30, 6.8, 5.9}, {112, 1.80, 5.2, 6.4}},
-                                    {{201, 1.70, 7.6, 3.6}, {172, 2.37, 4.7, 4.4}, {135, 3.64, 8.5, 6.8}}};
+                                    {{143, 0.77, 9.5, 5.9}, {185, 1.89, 5.3, 5.3}, {167, 3.73, 2.7, 5.4}}};
     const GroupedShape g(T_rows, E, N, K * (int64_t)sizeof(T));
     auto least = [&](double us, double inner, double outer) {  // not below the matrices' reading
         const double read = g.stream(y_inner ? inner : outer);
@@ -73,7 +74,7 @@ int choose_gmm_tile(int64_t T_rows, int64_t E, int64_t N, int64_t K, bool y_inne
         if (us < best_us) best = tile, best_us = us;
     };
     for (int i = 0; i < 3; ++i) consider(2 + i, least(estimate(g, kFew[F32][i], 1 << i), 4.8, 5.2));
-    if (!F32) consider(5, least(estimate(g, kBig), 4.2, 5.4));
+    consider(5, least(F32 ? estimate(g, kSmall) : estimate(g, kBig), 4.2, 5.4));
     if (us) *us = best_us;
     return best;
 }
@@ -203,6 +204,10 @@ int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &
         if (tile == 5)
             return aligned ? launch_gmm_tile<T, XL, YL, 256, 256, 2, 4, true, XL == kInner>(g, E, T_rows, s)
                            : launch_gmm_tile<T, XL, YL, 256, 256, 2, 4, false, XL == kInner>(g, E, T_rows, s);
+    } else if constexpr (XL == kInner) {
+        if (tile == 5)
+            return aligned ? launch_gmm_tile<T, XL, YL, 64, 64, 2, 2, true>(g, E, T_rows, s)
+                           : launch_gmm_tile<T, XL, YL, 64, 64, 2, 2, false>(g, E, T_rows, s);
     }
     return aligned ? launch_gmm_tile<T, XL, YL, 128, 128, 2, 2, true>(g, E, T_rows, s)
                    : launch_gmm_tile<T, XL, YL, 128, 128, 2, 2, false>(g, E, T_rows, s);

@@ -132,6 +132,21 @@ __device__ __forceinline__ bool find_tile(const Sizes &s, uint32_t wg, uint32_t 
     return false;
 }
 
+// Rows [row0, row0 + rows) of the group that stands at place e by length, the longest first, and its number; up to 64 groups.
+__device__ __forceinline__ uint32_t group_by_length(const Sizes &s, uint32_t e, int64_t &row0, int64_t &rows) {
+    uint32_t before = 0, start = 0, end = 0, place = 0;
+    chunk_rows(s, 0, before, start, end);
+    const uint32_t mine = (uint32_t)lane_id() < s.E ? end - start : 0;
+    for (uint32_t i = 0; i < s.E; ++i) {
+        const uint32_t other = lane_value(mine, i);
+        place += other > mine || (other == mine && i < (uint32_t)lane_id());
+    }
+    const int who = __builtin_ctzll(__ballot(place == e && (uint32_t)lane_id() < s.E));
+    row0 = lane_value(start, who);
+    rows = lane_value(end, who) - row0;
+    return who;
+}
+
 // Rows [row0, row0 + rows) of one group.
 __device__ __forceinline__ void group_rows(const Sizes &s, uint32_t e, int64_t &row0, int64_t &rows) {
     uint32_t before = 0, start = 0, end = 0;

@@ -2,8 +2,8 @@
 //
 // The host knows T rows in E groups and not their sizes: tiles are counted as if groups were equal, with half a row tile
 // lost per group.  `steps` are 64 bytes of the contraction.  The constants are least-squares fits (logarithm of the time) to every
-// tile's time on random shapes of 1 to 8192 rows per group: 100 of bf16, 50 of fp32, 80 of the 4-bit format.  The least estimate's
-// tile is 2.9 %, 2.6 % and 1.7 % behind the best one on average (34 %, 28 % and 28 % on the worst shape).
+// tile's time on random shapes of 1 to 8192 rows per group: 100 of bf16, 100 of fp32, 80 of the 4-bit format.  The least estimate's
+// tile is 2.9 %, 2.5 % and 1.7 % behind the best one on average (34 %, 34 % and 28 % on the worst shape).
 #pragma once
 
 #include <math.h>
@@ -43,6 +43,15 @@ inline double estimate(const GroupedShape &g, const BigCost &c) {
     const double n = g.tiles(256, 256), full = floor(n / 256), rest = n - 256 * full;
     const double us = rest <= 0 ? 0 : rest <= 64 ? c.quarter : rest <= 128 ? c.half : full > 0 ? c.whole : 0.75 * c.whole;
     return c.fixed + g.steps * (full * c.whole + us) + c.round * (full + (rest <= 0 ? 0 : rest <= 64 ? 0.4 : rest <= 128 ? 0.7 : 1));
+}
+
+// 64 x 64: a step of a workgroup alone, and its share of a CU that holds several.
+struct SmallCost {
+    double alone, shared, fixed;
+};
+inline double estimate(const GroupedShape &g, const SmallCost &c) {
+    const double each = c.shared * ceil(g.tiles(64, 64) / 256);
+    return c.fixed + g.steps * (each > c.alone ? each : c.alone);
 }
 
 // Few rows: 16 units of a workgroup's wavefronts one after the other, shared once more than `slots` workgroups are there, or the

@@ -78,7 +78,7 @@ def _forward(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor, tile: int = 
     T, K = a.shape
     E, _, N = b.shape
     dtype, dev = a.dtype, a.device
-    c = torch.empty((T, N), dtype=dtype, device=dev)
+    c = a.new_empty((T, N))
     if T == 0 or N == 0:
         return c
     if K == 0:
@@ -104,7 +104,7 @@ def _weights(a: torch.Tensor, g: torch.Tensor, sizes: torch.Tensor, tile: int = 
     T, K = a.shape
     E, N = sizes.shape[0], g.shape[1]
     dtype, dev = a.dtype, a.device
-    d = torch.empty((E, K, N), dtype=dtype, device=dev)
+    d = a.new_empty((E, K, N))
     if d.numel() == 0:
         return d
     if T == 0:
