@@ -250,3 +250,29 @@ def test_many_groups_and_saturating_sizes(dev):
     fit = torch.tensor([3] * 150 + [50] + [0] * 49, dtype=torch.int32, device=dev)
     assert torch.equal(gmm(a, b, s), gmm(a, b, fit))
     assert torch.equal(gmm_grad(g, a, b, s.long())[1], gmm_grad(g, a, b, fit)[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tile", range(1, 6))
+def test_neighbours_do_not_leak_from_any_tile(dev, tile, dtype):
+    """NaN next to a group's rows, in the next matrix and behind the last group: contractions and tiles that end inside a step
+    read none of it, with operands on and off 16-byte boundaries."""
+    from triturus_amd.gmm import _forward, _weights
+
+    for sizes, K, N in (([37, 0, 21, 64], 40, 56), ([37, 0, 21, 64], 41, 55), ([130, 1, 70, 3], 264, 328), ([300, 7, 10, 290], 333, 270)):
+        T = sum(sizes) + 9
+        for layout in ("kn", "nk"):
+            a, b, g = operands(dev, T, 4, K, N, dtype, layout)
+            s = torch.tensor(sizes, device=dev)
+            clean, grad = _forward(a, b, s, tile), _weights(a, g, s, tile)
+            lo, hi = sizes[0], sizes[0] + sizes[1] + sizes[2]
+            keep = torch.ones(T, dtype=torch.bool, device=dev)
+            if sizes[1] == 0:
+                a[lo:hi], g[lo:hi], b[2] = math.nan, math.nan, math.nan
+                keep[lo:hi] = False
+            b[1] = math.nan if sizes[1] == 0 else b[1]
+            a[T - 9:], g[T - 9:] = math.nan, math.inf
+            c, d = _forward(a, b, s, tile), _weights(a, g, s, tile)
+            assert torch.equal(c[keep], clean[keep]) and not c[T - 9:].any()
+            live = [0, 1, 3] if sizes[1] == 0 else [0, 1, 2, 3]
+            assert torch.equal(d[live], grad[live])

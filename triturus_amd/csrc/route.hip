@@ -50,16 +50,14 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// Whole numbers in the order of the values: 0 for -inf (never chosen), NaN above everything, -0 as 0.
+// Whole numbers in the order of the values, -0 as 0 and NaN above everything; up to kNever: -inf, never chosen.
+constexpr uint32_t kNever = 0x007fffffu;
 __device__ __forceinline__ uint32_t order_key(float x) {
-    x += 0.0f;
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    if (x != x) return 0xffffffffu;
-    if (u == 0xff800000u) return 0;
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __builtin_bit_cast(uint32_t, x != x ? __builtin_nanf("") : x + 0.0f);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t key) {
-    return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);  // 0xffffffff gives a NaN
+    return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
 // The lane's V logits of a row, -inf where there is none.
@@ -157,20 +155,18 @@ __global__ __launch_bounds__(kChooseThreads<V>) void route_choose_kernel(RouteAr
         int32_t expert = -1;
         float top = 0.0f;
         for (int j = 0; j < g.k; ++j) {
-            uint32_t best = 0;
-            int at = 0;
+            uint32_t best = key[0];
 #pragma unroll
-            for (int i = V - 1; i >= 0; --i) {
-                const bool up = key[i] >= best;
-                best = up ? key[i] : best;
-                at = up ? i : at;
-            }
+            for (int i = 1; i < V; ++i) best = key[i] > best ? key[i] : best;
             const uint32_t all = row_max(best);
+            int at = 0;  // the first place of it
+#pragma unroll
+            for (int i = V - 1; i >= 0; --i) at = key[i] == all ? i : at;
             const uint32_t holders = (uint32_t)(__ballot(best == all) >> shift) & 0xffff;
             const int winner = __builtin_ctz(holders);
             const int32_t index = __shfl(lane * V + at, shift + winner, kWave);
             if (j == 0) top = key_value(all);
-            if (all && lane == j) mine = all, expert = index;
+            if (all > kNever && lane == j) mine = all, expert = index;
 #pragma unroll
             for (int i = 0; i < V; ++i) key[i] = lane == winner && i == at ? 0 : key[i];
         }
@@ -311,7 +307,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
             const uint32_t key = order_key(x[i]);
             best = key > best ? key : best;
         }
-        const float top = key_value(row_max(best));
+        const float top = key_value(row_max(best));  // of a row of -inf: not used
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
