@@ -47,6 +47,33 @@ def test_gmm_statuses():
         assert weights(**bad) == -4, bad
 
 
+def test_gmm_grad_statuses():
+    lib = _lib.load()
+
+    def call(g=one, a=one, b=one, s=one, da=one, db=one, T=4, E=2, K=8, N=16, ldg=16, lda=8, st=i64(128, 16, 1), dtype=BF16, ws=null):
+        return lib.trt_gmm_grad(g, a, b, s, da, db, T, E, K, N, ldg, lda, st, dtype, 0, ws, 0, null)
+
+    for bad in (dict(g=null), dict(a=null), dict(b=null), dict(s=null), dict(da=null), dict(db=null), dict(T=0), dict(N=0), dict(dtype=1), dict(st=None)):
+        assert call(**bad) == -1, bad
+    for bad in (dict(ldg=-1), dict(lda=-1), dict(st=i64(128, 16, 3)), dict(ws=c_void_p(8))):
+        assert call(**bad) == -2, bad
+    for bad in (dict(T=1 << 31), dict(lda=1 << 22), dict(st=i64(128, 1 << 22, 1))):
+        assert call(**bad) == -4, bad
+    at = c_void_p(1 << 20)
+    assert lib.trt_gmm_grad_workspace_bytes(at, at, at, 16384, 8, 2048, 2048, 2048, 2048, i64(1 << 22, 2048, 1), BF16) == 0
+    assert lib.trt_gmm_grad_workspace_bytes(at, at, at, 16384, 8, 2049, 2048, 2048, 2049, i64(2049 * 2048, 2048, 1), BF16) == 16384 * 2056 * 2
+
+
+def test_capture_is_refused_by_name(monkeypatch):
+    from triturus_amd import gmm as module
+
+    monkeypatch.setattr(module, "_is_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="gmm_grad"):
+        module.refuse_capture("gmm")
+    monkeypatch.setattr(module, "_is_capturing", lambda: False)
+    module.refuse_capture("gmm")
+
+
 def test_gmm_workspace_is_for_operands_off_the_boundaries():
     lib = _lib.load()
     at = c_void_p(1 << 20)

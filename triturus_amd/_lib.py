@@ -104,6 +104,14 @@ SIGNATURES = {
     ),
     "trt_gmm_weights_workspace_bytes": (
         c_size_t, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
+    "trt_gmm_grad": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+         POINTER(c_int64), c_int, c_int, c_void_p, c_size_t, c_void_p],
+    ),
+    "trt_gmm_grad_workspace_bytes": (
+        c_size_t,
+        [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, POINTER(c_int64), c_int]),
     "trt_mx4_quantize": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "trt_mx4_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "trt_mx4_mm": (

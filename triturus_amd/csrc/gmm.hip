@@ -81,3 +81,26 @@ extern "C" size_t trt_gmm_weights_workspace_bytes(const void *a, const void *g, 
     weights_product(a, g, nullptr, nullptr, T, E, K, N, lda, ldg, dtype, 0, tile, {nullptr, 0, &bytes}, nullptr);
     return bytes;
 }
+
+// Both gradients in one call: the rows' product with b's last two axes exchanged, then the weights' product, which may use the same
+// workspace after it.
+extern "C" int trt_gmm_grad(const void *g, const void *a, const void *b, const void *sizes, void *da, void *db, int64_t T, int64_t E,
+                            int64_t K, int64_t N, int64_t ldg, int64_t lda, const int64_t sb[3], int dtype, int wide_sizes, void *workspace,
+                            size_t workspace_bytes, void *stream) {
+    if (!sb || !db) return TRT_E_INVALID;
+    const int64_t st[3] = {sb[0], sb[2], sb[1]};
+    size_t none = 0;  // the second product's arguments are looked at before the first is enqueued
+    int status = weights_product(a, g, sizes, db, T, E, K, N, lda, ldg, dtype, wide_sizes, 0, {workspace, workspace_bytes, &none}, stream);
+    if (!status) status = rows_product(g, b, sizes, da, T, E, N, K, ldg, st, dtype, wide_sizes, 0, {workspace, workspace_bytes, nullptr}, stream);
+    if (!status) status = weights_product(a, g, sizes, db, T, E, K, N, lda, ldg, dtype, wide_sizes, 0, {workspace, workspace_bytes, nullptr}, stream);
+    return status;
+}
+
+extern "C" size_t trt_gmm_grad_workspace_bytes(const void *g, const void *a, const void *b, int64_t T, int64_t E, int64_t K, int64_t N,
+                                               int64_t ldg, int64_t lda, const int64_t sb[3], int dtype) {
+    if (!sb) return 0;
+    const int64_t st[3] = {sb[0], sb[2], sb[1]};
+    const size_t rows = trt_gmm_workspace_bytes(g, b, T, E, N, K, ldg, st, dtype, 0);
+    const size_t weights = trt_gmm_weights_workspace_bytes(a, g, T, E, K, N, lda, ldg, dtype, 0);
+    return rows > weights ? rows : weights;
+}

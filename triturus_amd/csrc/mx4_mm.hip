@@ -306,7 +306,7 @@ __global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
 // 64 bytes of codes (4 blocks) by 64 columns: lane (n, g) takes block g of columns n, n + 16, .. and a column's 4 scale
 // bytes as one word.  A: the type of a's values, which the lane quantises itself on the way (32 neighbours of a
 // row: no other lane is needed, and a call is one launch), or uint8_t for codes.
-// FAST: at least 4 blocks in a row, and whole ones of values.
+// FAST: at least 4 blocks in a row.
 template <typename A, int RT, bool FAST, int CW = 4, int W = 8, int D = 2>
 __global__ __launch_bounds__(64 * W) void mx4_few_kernel(Mx4Args g) {
     constexpr int COLS = 16 * CW;
@@ -327,7 +327,6 @@ __global__ __launch_bounds__(64 * W) void mx4_few_kernel(Mx4Args g) {
         for (int j = 0; j < CW; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
     constexpr bool VALUES = sizeof(A) != 1;
-    static_assert(FAST || !VALUES, "values are quantised where all blocks are whole");
     struct Unit {
         A x[RT][VALUES ? 32 : 16];
         uint32_t sx[RT];
@@ -348,6 +347,8 @@ __global__ __launch_bounds__(64 * W) void mx4_few_kernel(Mx4Args g) {
                 if constexpr (VALUES) {
                     const int64_t k = u * 128 + gk * 32;
                     __builtin_memcpy(n.x[i], x + r * g.lda + (k < g.K - 32 ? k : g.K - 32), sizeof(n.x[i]));
+                    if (u * 128 < g.K && u * 128 + 128 > g.K)  // the unit where the row ends: its last block may not be whole
+                        if (k < g.K && k + 32 > g.K) load_values(x + r * g.lda + k, g.K - k, n.x[i]);
                 } else {
                     __builtin_memcpy(n.x[i], reinterpret_cast<const uint8_t *>(x) + r * g.lda + (at < bytes - 16 ? at : bytes - 16), 16);
                     __builtin_memcpy(&n.sx[i], sx + r * g.ldsa + word, 4);
@@ -364,8 +365,13 @@ __global__ __launch_bounds__(64 * W) void mx4_few_kernel(Mx4Args g) {
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 const int r = 16 * i + m;
-                load_values(x + r * g.lda + u * 64 + gk * 16, r < rows ? left : 0, n.x[i]);
-                n.sx[i] = load_scales4(sx + r * g.ldsa + u * 4, r < rows ? blocks : 0);
+                if constexpr (VALUES) {
+                    const int64_t k = u * 128 + gk * 32;
+                    load_values(x + r * g.lda + k, r < rows ? g.K - k : 0, n.x[i]);
+                } else {
+                    load_values(x + r * g.lda + u * 64 + gk * 16, r < rows ? left : 0, n.x[i]);
+                    n.sx[i] = load_scales4(sx + r * g.ldsa + u * 4, r < rows ? blocks : 0);
+                }
             }
 #pragma unroll
             for (int j = 0; j < CW; ++j) {
@@ -447,35 +453,37 @@ int launch_mx4_few(Mx4Args g, hipStream_t s) {
 // 16 rows a tile: more and smaller pieces where there are fewer tiles than CUs.
 template <typename A>
 int launch_mx4_few_rows(const Mx4Args &g, hipStream_t s) {
+    if (g.bytes < 64) return launch_mx4_few<A, 1, false>(g, s);
     const double n = GroupedShape(g.sizes.T, g.sizes.E, g.N, 64).tiles(16, kFewCols);
     if (n <= 64) return launch_mx4_few<A, 1, true, 1, 8, 4>(g, s);
     if (n <= 128) return launch_mx4_few<A, 1, true, 2, 8, 4>(g, s);
     return launch_mx4_few<A, 1, true>(g, s);
 }
 
+// The few-row kernel quantises a's values itself where its workgroups are few: each makes the codes of its rows again, which costs
+// less than a launch up to about a round of workgroups (2 rows, one matrix of 3392 x 4672: 15.0 us a call, 12.4 from
+// codes; 8 groups of 6 rows, 7328 x 416: 32 and 17, and the launch takes 2.3 on the GPU and 3 on the host).
+inline bool quantizes_on_the_way(int64_t T, int64_t E, int64_t N, int a_type, int tile) {
+    return a_type >= 0 && tile == 2 && GroupedShape(T, E, N, 64).tiles(16, kFewCols) <= 300;
+}
+
 // Tiles: 1 = 128 x 128, 2, 3 = 16, 32 rows x 64 columns of the few-row kernel, 4 = 256 x 256 (c of 16-bit types); the least of
-// the estimated times (tile_cost.hpp).
-inline int choose_mx4_tile(int64_t T, int64_t E, int64_t K, int64_t N, int dtype, int tile) {
+// the estimated times (tile_cost.hpp), with a launch more where values are quantised before.
+inline int choose_mx4_tile(int64_t T, int64_t E, int64_t K, int64_t N, int a_type, int dtype, int tile) {
     if (tile) return tile;
     constexpr MidCost kMid = {0.410, 0.740, 1.634, 4.7, 7.4};
     constexpr BigCost kBig = {0.897, 0.795, 0.445, 3.3, 7.7};
     constexpr FewCost kFew[2] = {{107, 1.10, 4.5, 6.3}, {127, 2.81, 2.7, 5.5}};
+    const double launch = a_type >= 0 ? 5.0 : 0.0;
     const GroupedShape g(T, E, N, ceil_div(K, 32) * 16);
     int best = 1;
-    double best_us = estimate(g, kMid);
+    double best_us = estimate(g, kMid) + launch;
     auto consider = [&](int t, double us) {
         if (us < best_us) best = t, best_us = us;
     };
-    for (int i = 0; i < 2; ++i) consider(2 + i, estimate(g, kFew[i], 1 << i));
-    if (dtype != TRT_F32) consider(4, estimate(g, kBig));
+    for (int i = 0; i < 2; ++i) consider(2 + i, estimate(g, kFew[i], 1 << i) + (quantizes_on_the_way(T, E, N, a_type, 2 + i) ? 0.0 : launch));
+    if (dtype != TRT_F32) consider(4, estimate(g, kBig) + launch);
     return best;
-}
-
-// The few-row kernel quantises a's values itself where its workgroups are few: each makes the codes of its rows again, which costs
-// less than a launch up to about a round of workgroups (2 rows, one matrix of 3392 x 4672: 15.0 us a call, 12.4 from
-// codes; 8 groups of 6 rows, 7328 x 416: 32 and 17, and the launch takes 2.3).
-inline bool quantizes_on_the_way(int64_t T, int64_t E, int64_t K, int64_t N, int tile) {
-    return tile == 2 && K % 32 == 0 && K >= 128 && GroupedShape(T, E, N, 64).tiles(16, kFewCols) <= 300;
 }
 
 template <typename T>
@@ -496,7 +504,7 @@ using namespace trt;
 
 extern "C" size_t trt_mx4_mm_workspace_bytes(int64_t T, int64_t E, int64_t K, int64_t N, int a_type, int dtype, int tile) {
     if (a_type < 0 || T <= 0 || E <= 0 || K <= 0 || N <= 0) return 0;
-    if (quantizes_on_the_way(T, E, K, N, choose_mx4_tile(T, E, K, N, dtype, tile))) return 0;
+    if (quantizes_on_the_way(T, E, N, a_type, choose_mx4_tile(T, E, K, N, a_type, dtype, tile))) return 0;
     return (size_t)(T * ceil_div(K, 32) * 17);
 }
 
@@ -515,7 +523,7 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
     constexpr int64_t kMost = (int64_t)1 << 23;
     if (sa[0] >= kMost || sb[1] >= kMost || N >= kMost || K > 2 * kMost || T >= (int64_t)1 << 31 || E >= (int64_t)1 << 31) return TRT_E_RANGE;
     const size_t need = trt_mx4_mm_workspace_bytes(T, E, K, N, a_type, dtype, tile);
-    tile = choose_mx4_tile(T, E, K, N, dtype, tile);
+    tile = choose_mx4_tile(T, E, K, N, a_type, dtype, tile);
     if (need && (!workspace || workspace_bytes < need)) return TRT_E_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return TRT_E_LAYOUT;
     Mx4Args g = {};
@@ -534,13 +542,12 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
         a_type = -1;
     }
     if (tile == 2 || tile == 3) {
-        const bool fast = g.bytes >= 64;
-        if (tile == 3) return fast ? launch_mx4_few<uint8_t, 2, true>(g, s) : launch_mx4_few<uint8_t, 2, false>(g, s);
+        if (tile == 3) return g.bytes >= 64 ? launch_mx4_few<uint8_t, 2, true>(g, s) : launch_mx4_few<uint8_t, 2, false>(g, s);
         switch (a_type) {
             case TRT_F32: return launch_mx4_few_rows<float>(g, s);
             case TRT_F16: return launch_mx4_few_rows<_Float16>(g, s);
             case TRT_BF16: return launch_mx4_few_rows<__bf16>(g, s);
-            default: return fast ? launch_mx4_few_rows<uint8_t>(g, s) : launch_mx4_few<uint8_t, 1, false>(g, s);
+            default: return launch_mx4_few_rows<uint8_t>(g, s);
         }
     }
     switch (dtype) {

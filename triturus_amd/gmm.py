@@ -135,6 +135,7 @@ class _Gmm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
+        refuse_capture("gmm")
         a, b, sizes = ctx.saved_tensors
         da = _forward(g, b.transpose(1, 2), sizes) if ctx.needs_input_grad[0] else None
         db = _weights(a, g, sizes) if ctx.needs_input_grad[1] else None
@@ -156,5 +157,25 @@ def gmm_grad(g: torch.Tensor, a: torch.Tensor, b: torch.Tensor, sizes: torch.Ten
     _check(a, b, sizes)
     assert g.shape == (a.shape[0], b.shape[2])
     assert g.dtype == a.dtype and g.device == a.device
-    with torch.no_grad():
-        return _forward(g, b.transpose(1, 2), sizes), _weights(a, g, sizes)
+    T, K = a.shape
+    E, _, N = b.shape
+    if not (T and K and N):
+        with torch.no_grad():
+            return _forward(g, b.transpose(1, 2), sizes), _weights(a, g, sizes)
+    dev = a.device
+    da, db = a.new_empty((T, K)), a.new_empty((E, K, N))
+    g, a, b, sizes = _rows(g), _rows(a), _matrices(b), sizes.contiguous()
+    lib, code = _lib.load(), _lib.DTYPE_CODES[a.dtype]
+    pg, pa, pb, ldg, lda, sb = g.data_ptr(), a.data_ptr(), b.data_ptr(), g.stride(0), a.stride(0), _lib.strides3(b)
+    ws_ptr, nbytes, ws = None, 0, None
+    if (pg | pa | pb) & 15 or (K | N | ldg | lda | sb[0] | (sb[2] if sb[1] == 1 else sb[1])) & 7:  # then a copy may pay
+        nbytes = lib.trt_gmm_grad_workspace_bytes(pg, pa, pb, T, E, K, N, ldg, lda, sb, code)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws_ptr = ws.data_ptr()
+    with _lib.on_device(dev):
+        status = lib.trt_gmm_grad(pg, pa, pb, sizes.data_ptr(), da.data_ptr(), db.data_ptr(), T, E, K, N, ldg, lda, sb, code,
+                                  sizes.dtype is torch.int64, ws_ptr, nbytes, _lib.raw_stream(dev))
+    if status:
+        _lib.check(status, "trt_gmm_grad")
+    return da, db

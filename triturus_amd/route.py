@@ -105,6 +105,7 @@ class _Route(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, *_):
+        refuse_capture("route")
         return _grad(g, *ctx.saved_tensors, ctx.normalize), None, None
 
 
