@@ -194,20 +194,22 @@ __device__ __forceinline__ void store_tile(const floatx16 (&acc)[RT][CT], char *
 }
 
 // Asks the scheduler for the block's instructions in turn: LDS writes, loads, LDS reads, MFMAs, an eighth of each at a time.
-template <int WRITES, int READS, int MFMAS, int... Q>
+template <int WRITES, int LOADS, int READS, int MFMAS, int... Q>
 __device__ __forceinline__ void interleave(std::integer_sequence<int, Q...>) {
-    constexpr int G = sizeof...(Q);
     auto part = [](auto q) {
-        constexpr int i = decltype(q)::value;
-        constexpr int w = WRITES * (i + 1) / G - WRITES * i / G, r = READS * (i + 1) / G - READS * i / G, m = MFMAS * (i + 1) / G - MFMAS * i / G;
-        if constexpr (w > 0) {
-            __builtin_amdgcn_sched_group_barrier(0x200, w, 0);
-            __builtin_amdgcn_sched_group_barrier(0x020, w, 0);
-        }
+        constexpr int i = decltype(q)::value, G = sizeof...(Q);
+        constexpr int w = WRITES * (i + 1) / G - WRITES * i / G, l = LOADS * (i + 1) / G - LOADS * i / G;
+        constexpr int r = READS * (i + 1) / G - READS * i / G, m = MFMAS * (i + 1) / G - MFMAS * i / G;
+        if constexpr (w > 0) __builtin_amdgcn_sched_group_barrier(0x200, w, 0);
+        if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x020, l, 0);
         if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
         if constexpr (m > 0) __builtin_amdgcn_sched_group_barrier(0x008, m, 0);
     };
     (part(std::integral_constant<int, Q>()), ...);
+}
+template <int WRITES, int LOADS, int READS, int MFMAS>
+__device__ __forceinline__ void interleave() {
+    interleave<WRITES, LOADS, READS, MFMAS>(std::make_integer_sequence<int, 8>());
 }
 
 struct GmmArgs {
@@ -295,8 +297,8 @@ __device__ __forceinline__ void gmm_tile(const T *x, int64_t ldx, const T *y, in
 #pragma unroll
                     for (int j = 0; j < CT; ++j) acc[i][j] = Mfma<T>::step(yf[kk & 1][j], xf[kk & 1][i], acc[i][j]);
                 if constexpr (ALIGNED) {
-                    if (kk == kSub - 1) interleave<X::N + Y::N, READS, MFMAS>(std::make_integer_sequence<int, 8>());
-                    else interleave<0, READS, MFMAS>(std::make_integer_sequence<int, 8>());
+                    if (kk == kSub - 1) interleave<X::N + Y::N, X::N + Y::N, READS, MFMAS>();
+                    else interleave<0, 0, READS, MFMAS>();
                 }
             }
             lds_barrier();
@@ -465,10 +467,11 @@ __device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T
         auto step = [&](int64_t s, const char *now, const char *next, char *fill) {
             fragments(now, 1);
             multiply(0);
-            interleave<0, READS, RT * CT>(std::make_integer_sequence<int, 8>());
+            interleave<0, 0, READS, RT * CT>();
             load(s + 3, fill);
             fragments(next, 0);
             multiply(1);
+            interleave<0, X::N + Y::N, READS, RT * CT>();
             direct_barrier<X::N + Y::N>();  // the loads of the step after next have landed
         };
         load(0, st0);
@@ -493,7 +496,7 @@ __device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T
 
 // CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT>
-__global__ __launch_bounds__(64 * WM *WN, (BM * BN / (WM * WN) > 4096 && WM * WN == 4) ? 2 : 1) void gmm_kernel(GmmArgs g) {
+__global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
     static_assert(!CUT || (BM == 256 && BN == 256 && WM == 2 && WN == 4 && XL == kInner), "the parts below");
     constexpr bool DIRECT = ALIGNED && BM == 256 && sizeof(T) == 2;
     constexpr int STAGE = DIRECT ? 512 * kStepBytes : 16;

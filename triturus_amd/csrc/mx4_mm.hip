@@ -144,7 +144,7 @@ __device__ __forceinline__ void mx4_tile(const Mx4Args &g, const uint8_t *x, con
                 for (int i = 0; i < RT; ++i)
 #pragma unroll
                     for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<0>(yf[0][j], ye[u & 1][j], xf[0][i], xe[u & 1][i], acc[i][j]);
-                if constexpr (ALIGNED) interleave<0, RT + CT, RT * CT>(std::make_integer_sequence<int, 8>());
+                if constexpr (ALIGNED) interleave<0, 0, RT + CT, RT * CT>();
                 store(after);  // the step that was read last: everyone is past the barrier behind it
                 if (u == 2) store_scales(s0 / 4 + 1);
                 load(s + 3);
@@ -154,7 +154,7 @@ __device__ __forceinline__ void mx4_tile(const Mx4Args &g, const uint8_t *x, con
                 for (int i = 0; i < RT; ++i)
 #pragma unroll
                     for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<1>(yf[1][j], ye[u & 1][j], xf[1][i], xe[u & 1][i], acc[i][j]);
-                if constexpr (ALIGNED) interleave<X::N + Y::N, 2 * (RT + CT), RT * CT>(std::make_integer_sequence<int, 8>());
+                if constexpr (ALIGNED) interleave<X::N + Y::N, X::N + Y::N, 2 * (RT + CT), RT * CT>();
                 lds_barrier();
                 char *const read = now;
                 now = next, next = after, after = read;
@@ -229,7 +229,7 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
             for (int i = 0; i < RT; ++i)
 #pragma unroll
                 for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<0>(yf[0][j], ye[U & 1][j], xf[0][i], xe[U & 1][i], acc[i][j]);
-            interleave<0, RT + CT, RT * CT>(std::make_integer_sequence<int, 8>());
+            interleave<0, 0, RT + CT, RT * CT>();
             load(s + 3, fill);
             if constexpr (U == 2) store_scales(s / 4 + 1);
             fragments(next, 0);
@@ -238,6 +238,7 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
             for (int i = 0; i < RT; ++i)
 #pragma unroll
                 for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<1>(yf[1][j], ye[U & 1][j], xf[1][i], xe[U & 1][i], acc[i][j]);
+            interleave<0, LOADS, 2 * (RT + CT), RT * CT>();
             direct_barrier<LOADS>();  // the loads of the step after next have landed
         };
         load(0, st0);
