@@ -142,8 +142,7 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Writes a finished tile: `out` is its first value, rows x cols of it exist, the output's rows are N long and start at
-// `base`.  acc[i][j][q] is row 32 i + (lane & 31), column 32 j + 8 (q / 4) + 4 (lane / 32) + q % 4 of the
+// Writes a finished tile: `out` is its first value, rows x cols of it exist, the output's rows are N long.  acc[i][j][q] is row 32 i + (lane & 31), column 32 j + 8 (q / 4) + 4 (lane / 32) + q % 4 of the
 // wavefront's part (the MFMA's first operand makes its rows, and that is Y here: 4 neighbours of an output row
 // in a lane).  The wavefront turns them round in LDS of its own and writes rows, 16 bytes a lane.
 template <typename T, int BM, int BN, int WM, int WN>
@@ -154,7 +153,7 @@ struct OutTile {
 
 template <typename T, int BM, int BN, int WM, int WN, int RT, int CT>
 __device__ __forceinline__ void store_tile(const floatx16 (&acc)[RT][CT], char *lds, int wave, T *out, int64_t N, int64_t rows,
-                                           int64_t cols, const void *base) {
+                                           int64_t cols) {
     constexpr int OUT_ROW = OutTile<T, BM, BN, WM, WN>::ROW;
     const int wm = wave / WN, wn = wave % WN, l = lane_id();
     char *mine = lds + wave * (BM / WM) * OUT_ROW;
@@ -174,22 +173,13 @@ __device__ __forceinline__ void store_tile(const floatx16 (&acc)[RT][CT], char *
     constexpr int V = 16 / sizeof(T), PER = BN / WN / V, STEP = kWave / PER;
     const int64_t wrows = rows - wm * (BM / WM), wcols = cols - wn * (BN / WN);
     T *dst = out + (int64_t)wm * (BM / WM) * N + wn * (BN / WN);
-    const bool whole = ((reinterpret_cast<uintptr_t>(base) | (uint64_t)(N * (int64_t)sizeof(T))) & 15) == 0;
     const int c = l % PER * V;
 #pragma unroll 4
     for (int r = l / PER; r < BM / WM; r += STEP) {
         if (r >= wrows || c >= wcols) continue;
         const uintx4 v = *reinterpret_cast<const uintx4 *>(mine + r * OUT_ROW + c * sizeof(T));
         T *p = dst + (int64_t)r * N + c;
-        if (whole) {
-            *reinterpret_cast<uintx4 *>(p) = v;
-        } else {
-            T e[V];
-            __builtin_memcpy(e, &v, 16);
-#pragma unroll
-            for (int u = 0; u < V; ++u)
-                if (c + u < wcols) p[u] = e[u];
-        }
+        store_chunk(p, v, wcols - c);
     }
 }
 
@@ -230,11 +220,10 @@ struct GmmLds {
     static constexpr int BYTES = kStages * STAGE > OUT ? kStages * STAGE : OUT;
 };
 
-// One tile: x, y and out at its first values, rows x cols of it exist, `terms` contracted values; `base`: where out's rows of N
-// start.
+// One tile: x, y and out at its first values, rows x cols of it exist, `terms` contracted values.
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED>
 __device__ __forceinline__ void gmm_tile(const T *x, int64_t ldx, const T *y, int64_t ldy, T *out, int64_t N, int64_t rows, int64_t cols,
-                                         int64_t terms, const void *base, char *lds) {
+                                         int64_t terms, char *lds) {
     constexpr int THREADS = 64 * WM * WN, RT = BM / WM / 32, CT = BN / WN / 32;
     using X = Operand<T, XL, BM, THREADS>;
     using Y = Operand<T, YL, BN, THREADS>;
@@ -306,7 +295,7 @@ __device__ __forceinline__ void gmm_tile(const T *x, int64_t ldx, const T *y, in
             now = next, next = after, after = read;
         }
     }
-    store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, N, rows, cols, base);
+    store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, N, rows, cols);
 }
 
 // ---- 256 x 256 tiles of aligned 16-bit operands: memory to LDS without registers between ----------------------------
@@ -387,9 +376,8 @@ __device__ __forceinline__ void direct_barrier() {
 // row r at c ^ (r % PER).  acc as for store_tile.
 template <typename T, int RT, int CT>
 __device__ __forceinline__ void store_direct(const floatx16 (&acc)[RT][CT], char *lds, int wave, int wm, int wn, T *out, int64_t N, int64_t rows,
-                                             int64_t cols, const void *base) {
+                                             int64_t cols) {
     constexpr int V = 8, PER = CT * 4, STEP = kWave / PER;
-    const bool whole = ((reinterpret_cast<uintptr_t>(base) | (uint64_t)(N * (int64_t)sizeof(T))) & 15) == 0;
     char *mine = lds + wave * (32 * CT * 32 * (int)sizeof(T));
     const int l = lane_id();
     const int64_t wcols = cols - wn * (CT * 32);
@@ -412,22 +400,14 @@ __device__ __forceinline__ void store_direct(const floatx16 (&acc)[RT][CT], char
             const uintx4 v = *reinterpret_cast<const uintx4 *>(mine + r * (PER * 16) + ((c ^ (r % PER)) * 16));
             if (row0 + r >= rows || c * V >= wcols) continue;
             T *p = out + (row0 + r) * N + wn * (CT * 32) + c * V;
-            if (whole) {
-                *reinterpret_cast<uintx4 *>(p) = v;
-            } else {
-                T e[V];
-                __builtin_memcpy(e, &v, 16);
-#pragma unroll
-                for (int u = 0; u < V; ++u)
-                    if (c * V + u < wcols) p[u] = e[u];
-            }
+            store_chunk(p, v, wcols - c * V);
         }
     }
 }
 
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN>
 __device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T *y, int64_t ldy, T *out, int64_t N, int64_t rows, int64_t cols,
-                                                int64_t terms, const void *base, char *st0, char *st1, char *st2, char *st3) {
+                                                int64_t terms, char *st0, char *st1, char *st2, char *st3) {
     constexpr int RT = BM / WM / 32, CT = BN / WN / 32;
     using X = Direct<T, XL, BM, WM * WN>;
     using Y = Direct<T, YL, BN, WM * WN>;
@@ -491,7 +471,7 @@ __device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T
         }
         direct_barrier<0>();  // nothing is on its way to LDS any more
     }
-    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, N, rows, cols, base);
+    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, N, rows, cols);
 }
 
 // CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
@@ -504,8 +484,8 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
     __shared__ __attribute__((aligned(16))) char lds[DIRECT ? 16 : GmmLds<T, XL, YL, BM, BN, WM, WN>::BYTES];
     auto tile = [&](auto bm, auto bn, auto wm, auto wn, const T *x, const T *y, T *out, int64_t rows, int64_t cols, int64_t terms) {
         constexpr int M = decltype(bm)::value, N = decltype(bn)::value, P = decltype(wm)::value, Q = decltype(wn)::value;
-        if constexpr (DIRECT) gmm_direct_tile<T, XL, YL, M, N, P, Q>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, g.out, st0, st1, st2, st3);
-        else gmm_tile<T, XL, YL, M, N, P, Q, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, g.out, lds);
+        if constexpr (DIRECT) gmm_direct_tile<T, XL, YL, M, N, P, Q>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, st0, st1, st2, st3);
+        else gmm_tile<T, XL, YL, M, N, P, Q, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, lds);
     };
     constexpr std::integral_constant<int, BM> bm;
     constexpr std::integral_constant<int, BN> bn;

@@ -93,10 +93,11 @@ int choose_weights_tile(int64_t E, int64_t K, int64_t N) {
 }
 
 // ---- operands off the 16-byte boundaries -------------------------------------------------------------------------------
-// Rows that start off them, or are not whole chunks, cost every product about twice its time (16-byte loads from any address, and no
-// loads to LDS) and the weights' gradient three times.  Where that is more than a copy, an operand is first copied into
-// rows of whole chunks with zeros behind (16384 rows in 8 groups, K = 2049, N = 2047: 354 us, 210 with both copied; the weights'
-// gradient 508 and 200).
+// Rows that start off them, or are not whole chunks, cost up to twice a product's time (16-byte loads from any address, and no
+// loads to LDS), least where both operands lie along the contraction, and the weights' gradient two to three times.  Where that
+// is more than a copy, an operand is first copied into rows of whole chunks with zeros behind (16384 rows in 8 groups of fp16,
+// K = 2049, N = 2047: 336 us as they are and 205 with both copied; matrices stored N x K 261 and 225; the weights' gradient
+// 500 and 191.  On the boundaries they take 157 to 180).
 
 // Rows of n values, `rows` to a group, strides in values, to dense rows of whole chunks.
 struct PadJob {
@@ -181,7 +182,7 @@ int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &
     }
     // few rows are bound by reading the matrices, and a copy reads and writes them
     const bool few = XL == kInner && tile >= 2 && tile <= 4;
-    const PadPlan pads = few ? PadPlan{false, false, 0} : plan_pads<T, XL, YL>(g, E, T_rows, us, XL == kOuter ? 1.2 : 0.8);
+    const PadPlan pads = few ? PadPlan{false, false, 0} : plan_pads<T, XL, YL>(g, E, T_rows, us, XL == kOuter ? 1.2 : YL == kOuter ? 0.8 : 0.5);
     if (w.query) {
         *w.query = pads.bytes;
         return TRT_OK;

@@ -192,5 +192,19 @@ __device__ __forceinline__ uintx4 load_chunk(const T *p, int64_t left) {
     }
     return v;
 }
+// The same way back: `left` > 0 values of the row from p on.
+template <typename T>
+__device__ __forceinline__ void store_chunk(T *p, uintx4 v, int64_t left) {
+    constexpr int V = 16 / sizeof(T);
+    if (left >= V) {
+        __builtin_memcpy(p, &v, 16);
+    } else {
+        T e[V];
+        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int i = 0; i < V - 1; ++i)
+            if (i < left) p[i] = e[i];
+    }
+}
 
 }  // namespace trt

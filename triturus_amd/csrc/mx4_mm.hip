@@ -161,7 +161,7 @@ __device__ __forceinline__ void mx4_tile(const Mx4Args &g, const uint8_t *x, con
             }
         }
     }
-    store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, g.N, rows, cols, g.out);
+    store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, g.N, rows, cols);
 }
 
 // 256 x 256 tiles (and their parts) of codes at 16-byte boundaries: codes from memory to LDS without registers between
@@ -261,7 +261,7 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
         }
         direct_barrier<0>();  // nothing is on its way to LDS any more
     }
-    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, g.N, rows, cols, g.out);
+    store_direct<T, RT, CT>(acc, st0, wave, wm, wn, out, g.N, rows, cols);
 }
 
 // CUT: 256 x 256 tiles whose last, short round is cut into halves or quarters (find_tile).
