@@ -3,19 +3,25 @@
 //   rows:     c[r, n] = sum_k a[r, k] b[e(r), k, n]     contraction of K terms, the same for every group
 //   weights:  d[e, k, n] = sum_{r in e} a[r, k] g[r, n] contraction over the group's own rows
 //
-// Both walk the contraction in steps of 128 bytes per row of a tile (64 values of 16 bits, 32 of fp32).
+// Both walk the contraction in steps of 64 bytes per row of a tile (32 values of 16 bits, 16 of fp32).
 // X is the operand that makes the rows of the tile, Y the one that makes its columns; each comes in one of two
 // layouts: INNER, where the contracted axis is contiguous (a; b stored N x K), or OUTER, where the output's
 // axis is (b stored K x N; both operands of `weights`).  A tile is read from memory 16 bytes a lane into
-// registers one step ahead, written to the idle half of a double buffer in LDS during the current step's
+// registers ahead of its step, written to the idle one of three stages in LDS during the current step's
 // MFMAs, and read from there as MFMA operands:
-//   INNER  [row][8 chunks of 16 bytes], chunk c of row r at c ^ (r & 7): the 8 rows that a quarter-wave reads
-//          at once lie in 8 different chunks, so all banks work;
+//   INNER  [row][4 chunks of 16 bytes], chunk c of row r at c ^ (r / 4 % 4): four runs of 4 rows, whose chunks are in four
+//          different places, fill all 64 banks;
 //   OUTER  [contracted][row], 16-bit types by the transposing LDS read (ds_read_b64_tr_b16: 4 x 16 values per
-//          16 lanes, each lane gets one column), fp32 by 4-byte reads (32 neighbours); rows are 32 bytes
-//          longer than their data, so that the 4 rows of a transposing read lie in different banks.
+//          16 lanes, each lane gets one column), with row k's pairs of chunks turned by 2 (k % 4) so that the 4 rows and 2 pairs
+//          that are read at a time lie in all banks; fp32 by 4-byte reads (32 neighbours) from rows 32 bytes longer than
+//          their data.
+// (With r / 2 % 4 and turns by k % 4, half of the reads met in a bank: LDS was busy 52 % of the time on 256 x 256 tiles, 26 % so.)
 // Sums are fp32; a result is rounded once.  The finished tile goes through LDS, so that rows are
 // written 16 bytes a lane.
+//
+// Bound: the matrix pipe and, on 256 x 256 tiles, the card's power: 16384 rows in 8 groups, K = N = 4096 of bf16 take 513 us
+// (1072 TFLOP/s; the weights' gradient 454 us, 1212) with the pipe busy 64 % (67 %) of cycles that the clock has stretched to
+// 1.6 GHz.  128 x 128 tiles reach 797 TFLOP/s there (895), fp32 140 (one group of 4096 x 4096 x 4096).
 #pragma once
 
 #include <utility>
@@ -57,15 +63,18 @@ struct Operand {
     static constexpr int V = 16 / sizeof(T);           // values per chunk
     static constexpr int KT = kStepBytes / sizeof(T);  // contracted values per step
     static constexpr int CHUNKS = kStepBytes / 16;
-    static constexpr int ROW = LAYOUT == kInner ? kStepBytes : B * (int)sizeof(T) + 32;  // bytes of an LDS row
+    static constexpr int ROW = LAYOUT == kInner ? kStepBytes : B * (int)sizeof(T) + (sizeof(T) == 4 ? 32 : 0);  // bytes of an LDS row
     static constexpr int LDS = LAYOUT == kInner ? B * kStepBytes : KT * ROW;
     static constexpr int PER_ROW = LAYOUT == kInner ? CHUNKS : B / V;  // chunks per LDS row
     static constexpr int N = B * CHUNKS / THREADS;     // chunks per thread
     static constexpr int ROWS_STEP = THREADS / PER_ROW;
     static_assert(THREADS % PER_ROW == 0 && B * CHUNKS % THREADS == 0, "threads cover whole LDS rows");
 
-    // INNER: chunk c of row r lies at c ^ (r / 2 % 4), so that 8 neighbouring rows' chunks c lie in different banks
-    static __device__ __forceinline__ int place(int row, int c) { return row * ROW + ((c ^ ((row >> 1) & 3)) * 16); }
+    // Chunk c of a row of LDS.
+    static __device__ __forceinline__ int place(int row, int c) {
+        const int turn = LAYOUT == kInner ? (row >> 2) & 3 : sizeof(T) == 4 ? 0 : B >= 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
+        return row * ROW + ((c ^ turn) * 16);
+    }
 
     uintx4 reg[N];
 
@@ -105,9 +114,7 @@ struct Operand {
         const int r = tid / PER_ROW, c = tid % PER_ROW;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int row = r + i * ROWS_STEP;
-            const int at = LAYOUT == kInner ? place(row, c) : row * ROW + c * 16;
-            *reinterpret_cast<uintx4 *>(lds + at) = reg[i];
+            *reinterpret_cast<uintx4 *>(lds + place(r + i * ROWS_STEP, c)) = reg[i];
         }
     }
 
@@ -119,8 +126,8 @@ struct Operand {
         } else if constexpr (sizeof(T) == 2) {
             typedef short short4v __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) short4v *lds4;
-            const int k = 16 * kk + 8 * half + ((l & 15) >> 2), col = row + (m & 16) + 4 * (l & 3);
-            char *at = const_cast<char *>(lds) + k * ROW + col * 2;
+            const int k = 16 * kk + 8 * half + ((l & 15) >> 2);
+            char *at = const_cast<char *>(lds) + place(k, (row + (m & 16)) / 8) + 8 * (l & 3);  // turns are of whole pairs of chunks
             const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
             const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * ROW));
             const uintx2 a = __builtin_bit_cast(uintx2, lo), b = __builtin_bit_cast(uintx2, hi);
@@ -303,9 +310,8 @@ typedef __attribute__((address_space(3))) void *lds_ptr;
 
 // One operand's share of a 64-byte step, written by buffer loads that go to LDS: a wavefront's load fills 1 KiB there, lane by
 // lane, so the places are fixed and it is the lanes' sources that are permuted.
-//   INNER  [row][4 chunks], chunk c of row r at c ^ (r / 2 % 4);
-//   OUTER  [contracted][row], the 32 bytes p of contracted value k at p ^ (k % 4): a transposing read's 4 x 32 bytes lie in
-//          different banks.
+//   INNER  [row][4 chunks], chunk c of row r at c ^ (r / 4 % 4);
+//   OUTER  [contracted][row], the 32 bytes p of contracted value k at p ^ (2 (k % 4)).
 template <typename T, int LAYOUT, int B, int WAVES>
 struct Direct {
     static constexpr int KT = kStepBytes / sizeof(T);
@@ -323,11 +329,11 @@ struct Direct {
         for (int i = 0; i < N; ++i) {
             const int place = (wave * N + i) * 1024 + l * 16, row = place / ROW, slot = place % ROW / 16;
             if constexpr (LAYOUT == kInner) {
-                const int c = slot ^ ((row >> 1) & 3);
+                const int c = slot ^ ((row >> 2) & 3);
                 depth[i] = c * 8;
                 at[i] = row < out ? row * (uint32_t)(ld * sizeof(T)) + c * 16 : 0x80000000u;
             } else {
-                const int c = slot ^ (2 * (row & 3));
+                const int c = slot ^ (4 * (row & 3));
                 depth[i] = row;
                 at[i] = c * 8 < out ? row * (uint32_t)(ld * sizeof(T)) + c * 16 : 0x80000000u;
             }
@@ -347,12 +353,12 @@ struct Direct {
         const int l = lane_id(), half = l >> 5, m = l & 31;
         if constexpr (LAYOUT == kInner) {
             const int r = row + m;
-            return *reinterpret_cast<const uintx4 *>(stage + (base + r * ROW + (((2 * kk + half) ^ ((r >> 1) & 3)) * 16)));
+            return *reinterpret_cast<const uintx4 *>(stage + (base + r * ROW + (((2 * kk + half) ^ ((r >> 2) & 3)) * 16)));
         } else {
             typedef short short4v __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) short4v *lds4;
             const int k = 16 * kk + 8 * half + ((l & 15) >> 2), pair = row / 16 + (m >> 4);
-            const int at = base + k * ROW + ((pair ^ (k & 3)) * 32) + 8 * (l & 3);
+            const int at = base + k * ROW + ((pair ^ (2 * (k & 3))) * 32) + 8 * (l & 3);
             const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<char *>(stage + at));
             const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<char *>(stage + (at + 4 * ROW)));
             const uintx2 a = __builtin_bit_cast(uintx2, lo), b = __builtin_bit_cast(uintx2, hi);

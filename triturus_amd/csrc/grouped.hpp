@@ -76,7 +76,8 @@ __device__ __forceinline__ void chunk_rows(const Sizes &s, uint32_t e, uint32_t 
 //
 // CUT: tiles of which a CU holds one at a time run in rounds of kCus, and a last round of a few tiles would take as long as a
 // full one.  Up to kCus / 4 tiles of it are cut into quarters, up to kCus / 2 into halves, which then fill one shorter round
-// (8 groups of 16384 rows in all, K = N = 4096, 1088 tiles of 256 x 256: 560 us in 5 rounds, 520 with quarters).
+// (8 groups of 16384 rows in all, K = N = 4096, 1088 tiles of 256 x 256: 560 us in 5 rounds, 541 with
+// quarters, before later steps).
 constexpr uint32_t kCus = 256;
 template <int BM, bool CUT = false>
 __device__ __forceinline__ bool find_tile(const Sizes &s, uint32_t wg, uint32_t columns, GroupTile &t) {

@@ -5,7 +5,11 @@
 // bytes of a fragment are one block: v_mfma_scale_f32_32x32x64_f8f6f4 takes them with the block's scale byte and
 // multiplies and scales in one instruction at 4 times the rate of 16-bit operands.  Tiles, staging and LDS
 // layout are those of gmm.hpp (the INNER layout in bytes); the 4 scale bytes of a row's step go with them as
-// one word, from which a lane reads the two of its half: blocks 2 kk + (lane >= 32), kk = 0, 1.
+// one word, from which a lane reads the two of its half: blocks 2 kk + (lane >= 32), kk = 0, 1.  In LDS the words lie [step][row],
+// so that 32 rows' reads lie in different banks (16 bytes apart, as they come from memory, a dense product took 169 us, 158 so).
+//
+// Bound: as for 16-bit operands the card's power, and latency: 8192 x 4096 by 8192 x 4096 to bf16 takes 158 us (3485 TFLOP/s), the
+// matrix pipe busy 45 % of cycles at 1.9 GHz; 16384 rows in 8 groups, K = N = 4096, 190 us (2888).
 #include "few.hpp"
 #include "mx4.hpp"
 #include "tile_cost.hpp"
@@ -83,7 +87,7 @@ __device__ __forceinline__ void mx4_tile(const Mx4Args &g, const uint8_t *x, con
             const int64_t row = r < BM ? (r < rows ? r : rows - 1) : (r - BM < cols ? r - BM : cols - 1);
             sp[i] = r < BM ? sx + row * g.ldsa : sy + row * g.ldsb;
         }
-        char *const ring = lds + kStages * L::CODES;  // scales of four steps, and of the next four
+        char *const ring = lds + kStages * L::CODES;  // scales of four steps, [step][row], and of the next four
         auto load_scales = [&](int64_t q) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) scales[i] = load_chunk(sp[i] + q * 16, blocks - q * 16);
@@ -92,7 +96,9 @@ __device__ __forceinline__ void mx4_tile(const Mx4Args &g, const uint8_t *x, con
 #pragma unroll
             for (int i = 0; i < NS; ++i)
                 if (NS * THREADS == BM + BN || tid + i * THREADS < BM + BN)
-                    *reinterpret_cast<uintx4 *>(ring + (q & 1) * L::SCALES + (tid + i * THREADS) * 16) = scales[i];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        *reinterpret_cast<uint32_t *>(ring + (q & 1) * L::SCALES + (u * (BM + BN) + tid + i * THREADS) * 4) = scales[i][u];
         };
         auto load = [&](int64_t s) {  // behind the last step nothing remains, and nothing is read
             const int64_t left = bytes - s * kStepBytes;
@@ -112,14 +118,14 @@ __device__ __forceinline__ void mx4_tile(const Mx4Args &g, const uint8_t *x, con
             for (int j = 0; j < CT; ++j) yf[kk][j] = Y::fragment(from + X::LDS, (wn * CT + j) * 32, kk);
         };
         auto exponents = [&](int64_t s, int which) {
-            const char *e = ring + ((s >> 2) & 1) * L::SCALES + (s & 3) * 4;
+            const char *e = ring + ((s >> 2) & 1) * L::SCALES + (s & 3) * (BM + BN) * 4;
             const int half = 8 * (l >> 5);
 #pragma unroll
             for (int i = 0; i < RT; ++i)
-                xe[which][i] = *reinterpret_cast<const uint32_t *>(e + ((wm * RT + i) * 32 + (l & 31)) * 16) >> half;
+                xe[which][i] = *reinterpret_cast<const uint32_t *>(e + ((wm * RT + i) * 32 + (l & 31)) * 4) >> half;
 #pragma unroll
             for (int j = 0; j < CT; ++j)
-                ye[which][j] = *reinterpret_cast<const uint32_t *>(e + (BM + (wn * CT + j) * 32 + (l & 31)) * 16) >> half;
+                ye[which][j] = *reinterpret_cast<const uint32_t *>(e + (BM + (wn * CT + j) * 32 + (l & 31)) * 4) >> half;
         };
         load(0);
         load_scales(0);
@@ -200,7 +206,9 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
         uintx4 scales;
         auto load_scales = [&](int64_t q) { scales = load_chunk(sp + q * 16, blocks - q * 16); };
         auto store_scales = [&](int64_t q) {
-            if (BM + BN == 64 * WM * WN || tid < BM + BN) *reinterpret_cast<uintx4 *>(ring + ((q & 1) * SCALES + tid * 16)) = scales;
+            if (BM + BN < 64 * WM * WN && tid >= BM + BN) return;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) *reinterpret_cast<uint32_t *>(ring + ((q & 1) * SCALES + (u * (BM + BN) + tid) * 4)) = scales[u];
         };
         uintx4 xf[2][RT], yf[2][CT];
         uint32_t xe[2][RT], ye[2][CT];  // of this step and the next one, moved to the lane's half
@@ -211,13 +219,13 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
             for (int j = 0; j < CT; ++j) yf[kk][j] = Y::fragment(from, X::LDS, (wn * CT + j) * 32, kk);
         };
         auto exponents = [&](int64_t s, int which) {
-            const int e = (int)((s >> 2) & 1) * SCALES + (int)(s & 3) * 4, half = 8 * (l >> 5);
+            const int e = (int)((s >> 2) & 1) * SCALES + (int)(s & 3) * (BM + BN) * 4, half = 8 * (l >> 5);
 #pragma unroll
             for (int i = 0; i < RT; ++i)
-                xe[which][i] = *reinterpret_cast<const uint32_t *>(ring + (e + ((wm * RT + i) * 32 + (l & 31)) * 16)) >> half;
+                xe[which][i] = *reinterpret_cast<const uint32_t *>(ring + (e + ((wm * RT + i) * 32 + (l & 31)) * 4)) >> half;
 #pragma unroll
             for (int j = 0; j < CT; ++j)
-                ye[which][j] = *reinterpret_cast<const uint32_t *>(ring + (e + (BM + (wn * CT + j) * 32 + (l & 31)) * 16)) >> half;
+                ye[which][j] = *reinterpret_cast<const uint32_t *>(ring + (e + (BM + (wn * CT + j) * 32 + (l & 31)) * 4)) >> half;
         };
         static_assert(kSub == 2, "two sub-steps: the scale bytes 0 and 2 of the lane's half");
         // U: the step's place in its four.  The scales of the next four are asked for in the first and stored in the third.
