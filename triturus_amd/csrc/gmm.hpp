@@ -19,9 +19,9 @@
 // Sums are fp32; a result is rounded once.  The finished tile goes through LDS, so that rows are
 // written 16 bytes a lane.
 //
-// Bound: the matrix pipe and, on 256 x 256 tiles, the card's power: 16384 rows in 8 groups, K = N = 4096 of bf16 take 513 us
-// (1072 TFLOP/s; the weights' gradient 454 us, 1212) with the pipe busy 64 % (67 %) of cycles that the clock has stretched to
-// 1.6 GHz.  128 x 128 tiles reach 797 TFLOP/s there (895), fp32 140 (one group of 4096 x 4096 x 4096).
+// Bound: the matrix pipe and, on 256 x 256 tiles, the card's power: 16384 rows in 8 groups, K = N = 4096 of bf16 take 499 us
+// (1102 TFLOP/s; matrices stored N x K 520 us; the weights' gradient 441 us, 1246) with the pipe busy 69 % of cycles that the
+// clock has stretched to 1.55 GHz.  128 x 128 tiles reach 797 TFLOP/s there (895), fp32 140 (one group of 4096 x 4096 x 4096).
 #pragma once
 
 #include <utility>
@@ -450,30 +450,41 @@ __device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T
                 for (int j = 0; j < CT; ++j) acc[i][j] = Mfma<T>::step(yf[kk][j], xf[kk][i], acc[i][j]);
         };
         constexpr int XR = XL == kInner ? 1 : 2, YR = YL == kInner ? 1 : 2, READS = RT * XR + CT * YR;
-        auto step = [&](int64_t s, const char *now, const char *next, char *fill) {
+        constexpr int LOADS = X::N + Y::N;
+        // The barrier stands where the last reads of `now` are done: the loads of the step after the next three go there at once, and
+        // have three steps' time.
+        auto step = [&](int64_t s, char *now, const char *next) {
             fragments(now, 1);
             multiply(0);
             interleave<0, 0, READS, RT * CT>();
-            load(s + 3, fill);
+            direct_barrier<2 * LOADS>();  // the loads of the next step have landed
+            load(s + 4, now);
             fragments(next, 0);
             multiply(1);
-            interleave<0, X::N + Y::N, READS, RT * CT>();
-            direct_barrier<X::N + Y::N>();  // the loads of the step after next have landed
+            interleave<0, LOADS, READS, RT * CT>();
         };
         load(0, st0);
         load(1, st1);
         load(2, st2);
-        direct_barrier<X::N + Y::N>();
+        load(3, st3);
+        direct_barrier<3 * LOADS>();
         fragments(st0, 0);
-        for (int64_t s = 0;;) {
-            step(s, st0, st1, st3);
-            if (++s >= steps) break;
-            step(s, st1, st2, st0);
-            if (++s >= steps) break;
-            step(s, st2, st3, st1);
-            if (++s >= steps) break;
-            step(s, st3, st0, st2);
-            if (++s >= steps) break;
+        // One way out of the loop: with one behind each step, the compiler joined them before its head, took the loads of any stage
+        // to be on their way there, and waited for all of them every fourth step.  (With that, the barrier at the end of a step and
+        // half of the time for the loads, the sizes above took 513 us, and the weights' gradient 454.)
+        int64_t s = 0;
+        for (; s + 4 <= steps; s += 4) {
+            step(s, st0, st1);
+            step(s + 1, st1, st2);
+            step(s + 2, st2, st3);
+            step(s + 3, st3, st0);
+        }
+        if (s < steps) {
+            step(s, st0, st1);
+            if (s + 1 < steps) {
+                step(s + 1, st1, st2);
+                if (s + 2 < steps) step(s + 2, st2, st3);
+            }
         }
         direct_barrier<0>();  // nothing is on its way to LDS any more
     }

@@ -8,8 +8,8 @@
 // one word, from which a lane reads the two of its half: blocks 2 kk + (lane >= 32), kk = 0, 1.  In LDS the words lie [step][row],
 // so that 32 rows' reads lie in different banks (16 bytes apart, as they come from memory, a dense product took 169 us, 158 so).
 //
-// Bound: as for 16-bit operands the card's power, and latency: 8192 x 4096 by 8192 x 4096 to bf16 takes 158 us (3485 TFLOP/s), the
-// matrix pipe busy 45 % of cycles at 1.9 GHz; 16384 rows in 8 groups, K = N = 4096, 190 us (2888).
+// Bound: as for 16-bit operands the card's power, and latency: 8192 x 4096 by 8192 x 4096 to bf16 takes 158 us (3470 TFLOP/s), the
+// matrix pipe busy 46 % of cycles at 1.8 GHz; 16384 rows in 8 groups, K = N = 4096, 192 us (2860).
 #include "few.hpp"
 #include "mx4.hpp"
 #include "tile_cost.hpp"
@@ -229,7 +229,7 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
         };
         static_assert(kSub == 2, "two sub-steps: the scale bytes 0 and 2 of the lane's half");
         // U: the step's place in its four.  The scales of the next four are asked for in the first and stored in the third.
-        auto step = [&](auto u, int64_t s, const char *now, const char *next, char *fill) {
+        auto step = [&](auto u, int64_t s, char *now, const char *next) {
             constexpr int U = decltype(u)::value;
             if constexpr (U == 0) load_scales(s / 4 + 1);
             fragments(now, 1);
@@ -238,7 +238,8 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
 #pragma unroll
                 for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<0>(yf[0][j], ye[U & 1][j], xf[0][i], xe[U & 1][i], acc[i][j]);
             interleave<0, 0, RT + CT, RT * CT>();
-            load(s + 3, fill);
+            direct_barrier<2 * LOADS>();  // the loads of the next step have landed
+            load(s + 4, now);
             if constexpr (U == 2) store_scales(s / 4 + 1);
             fragments(next, 0);
             exponents(s + 1, ~U & 1);
@@ -247,25 +248,33 @@ __device__ __forceinline__ void mx4_direct_tile(const Mx4Args &g, const uint8_t 
 #pragma unroll
                 for (int j = 0; j < CT; ++j) acc[i][j] = mx4_mfma<1>(yf[1][j], ye[U & 1][j], xf[1][i], xe[U & 1][i], acc[i][j]);
             interleave<0, LOADS, 2 * (RT + CT), RT * CT>();
-            direct_barrier<LOADS>();  // the loads of the step after next have landed
         };
         load(0, st0);
         load_scales(0);
         store_scales(0);
         load(1, st1);
         load(2, st2);
-        direct_barrier<LOADS>();
+        load(3, st3);
+        direct_barrier<3 * LOADS>();
         fragments(st0, 0);
         exponents(0, 0);
-        for (int64_t s = 0;;) {
-            step(std::integral_constant<int, 0>(), s, st0, st1, st3);
-            if (++s >= steps) break;
-            step(std::integral_constant<int, 1>(), s, st1, st2, st0);
-            if (++s >= steps) break;
-            step(std::integral_constant<int, 2>(), s, st2, st3, st1);
-            if (++s >= steps) break;
-            step(std::integral_constant<int, 3>(), s, st3, st0, st2);
-            if (++s >= steps) break;
+        constexpr std::integral_constant<int, 0> u0;
+        constexpr std::integral_constant<int, 1> u1;
+        constexpr std::integral_constant<int, 2> u2;
+        constexpr std::integral_constant<int, 3> u3;
+        int64_t s = 0;  // one way out of the loop, as in gmm_direct_tile
+        for (; s + 4 <= steps; s += 4) {
+            step(u0, s, st0, st1);
+            step(u1, s + 1, st1, st2);
+            step(u2, s + 2, st2, st3);
+            step(u3, s + 3, st3, st0);
+        }
+        if (s < steps) {
+            step(u0, s, st0, st1);
+            if (s + 1 < steps) {
+                step(u1, s + 1, st1, st2);
+                if (s + 2 < steps) step(u2, s + 2, st2, st3);
+            }
         }
         direct_barrier<0>();  // nothing is on its way to LDS any more
     }
