@@ -276,3 +276,30 @@ def test_neighbours_do_not_leak_from_any_tile(dev, tile, dtype):
             assert torch.equal(c[keep], clean[keep]) and not c[T - 9:].any()
             live = [0, 1, 3] if sizes[1] == 0 else [0, 1, 2, 3]
             assert torch.equal(d[live], grad[live])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_rows_far_apart(dev, dtype):
+    """Rows of long sequences' last tokens, and matrices' rows, further apart than a tile's 31-bit offsets reach."""
+    far, K, N = (1 << 23) // torch.finfo(dtype).bits * 8 + 8, 40, 24  # values; one more chunk than the limit
+    a, b, g = operands(dev, 3, 2, K, N, dtype)
+    wide = [torch.empty(t.shape[0] if t.dim() == 2 else 2 * t.shape[1], far, dtype=dtype, device=dev) for t in (a, b, g)]
+    av, gv = wide[0][:, :K].copy_(a), wide[2][:, :N].copy_(g)
+    bv = wide[1].view(2, K, far)[:, :, :N].copy_(b)
+    for rows in (3, 1):
+        sizes = [rows - 1, 1]
+        for got, want in zip(check(av[:rows], bv, gv[:rows], sizes), check(a[:rows], b, g[:rows], sizes)):
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("sizes,N", [([300, 2, 500], 1500), ([300, 0, 1500, 700], 2000), ([900, 1100, 600, 700], 4000)])
+def test_rounds_of_the_largest_tile(dev, sizes, N, layout):
+    """Last rounds in quarters, in halves and behind whole ones, under contractions that end at every step of the loop."""
+    from triturus_amd.gmm import _forward, _weights
+
+    for K in (8, 64, 96, 128, 136, 256, 328):
+        a, b, g = operands(dev, sum(sizes) + 5, len(sizes), K, N, torch.bfloat16, layout)
+        s = torch.tensor(sizes, device=dev)
+        close(_forward(a, b, s, 5), product64(a, b, sizes), product64(a.abs(), b.abs(), sizes), K)
+    close(_weights(a, g, s, 5), weights64(a, g, sizes), weights64(a.abs(), g.abs(), sizes), max(sizes))

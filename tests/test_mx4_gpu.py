@@ -274,3 +274,34 @@ def test_few_rows_over_many_columns(dev, N):
             a = torch.randn(2, K, device=dev).to(dtype)
             c = check(a, b)
             assert torch.equal(mm_mx4(mx4_quantize(a), b, dtype=dtype), c)
+
+
+def test_rows_far_apart(dev):
+    """Rows further apart than a tile's 31-bit offsets reach, of values and of codes."""
+    far, K, N = (1 << 23) + 32, 96, 40
+    a, b = torch.randn(3, K, device=dev).bfloat16(), mx4_quantize(torch.randn(N, K, device=dev))
+    av = torch.empty(3, far, dtype=a.dtype, device=dev)[:, :K].copy_(a)
+    q = mx4_quantize(a)
+    qv = MX4(torch.empty(3, far, dtype=torch.uint8, device=dev)[:, :q.codes.shape[1]].copy_(q.codes), q.scales, K)
+    for rows in (3, 1):
+        want = mm_mx4(a[:rows], b)
+        assert torch.equal(mm_mx4(av[:rows], b), want)
+        assert torch.equal(mm_mx4(MX4(qv.codes[:rows], qv.scales[:rows], K), b), want)
+    assert torch.equal(mx4_dequantize(qv), mx4_dequantize(q)) and torch.equal(mx4_quantize(av).codes, q.codes)
+
+
+@pytest.mark.parametrize("sizes,N", [([300, 2, 500], 1500), ([300, 0, 1500, 700], 2000), ([900, 1100, 600, 700], 4000)])
+def test_rounds_of_the_largest_tile(dev, sizes, N):
+    """Last rounds in quarters, in halves and behind whole ones, under contractions that end at every step of the loop."""
+    T = sum(sizes) + 5
+    s = torch.tensor(sizes, device=dev)
+    for K in (32, 128, 256, 384, 512, 640, 1056, 1312):
+        a, b = mx4_quantize(torch.randn(T, K, device=dev)), mx4_quantize(torch.randn(len(sizes), N, K, device=dev))
+        c = mm_mx4(a, b, s, _tile=4)
+        av, bv = mx4_dequantize(a), mx4_dequantize(b)
+        want, size, r = torch.zeros(T, N, dtype=torch.float64, device=dev), torch.zeros(T, N, dtype=torch.float64, device=dev), 0
+        for e, n in enumerate(sizes):
+            want[r:r + n] = av[r:r + n].double() @ bv[e].double().T
+            size[r:r + n] = av[r:r + n].double().abs() @ bv[e].double().abs().T
+            r += n
+        close(c, want.cpu(), size.cpu(), K)

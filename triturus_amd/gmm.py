@@ -40,23 +40,33 @@ def refuse_capture(op: str) -> None:
         )
 
 
+# The kernels address 256 rows of a tile with 31-bit byte offsets: rows further apart than this many bytes are copied
+# (the last token of long sequences, ``h[:, -1]``).
+ROW_STRIDE_LIMIT = 1 << 23
+
+
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """A copy whose strides are those of its shape (``contiguous()`` keeps any stride of an axis of length one)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Rows with a unit trailing stride, in place where the tensor has them."""
     st = t.stride()
-    return t if (st[1] == 1 or t.shape[1] == 1) and st[0] >= 0 else t.contiguous()
+    return t if (st[1] == 1 or t.shape[1] == 1) and 0 <= st[0] * t.itemsize < ROW_STRIDE_LIMIT else dense(t)
 
 
 def _matrices(b: torch.Tensor) -> torch.Tensor:
     """Matrices with a unit stride along one of their axes, in place where the tensor has them."""
-    st = b.stride()
-    if (st[2] == 1 or st[1] == 1) and min(st) >= 0:
-        return b
+    st, most = b.stride(), ROW_STRIDE_LIMIT // b.itemsize
     if min(st) >= 0:
-        if b.shape[2] == 1:
+        if (st[1] == 1 and st[2] < most) or (st[2] == 1 and st[1] < most):
+            return b
+        if b.shape[2] == 1 and st[1] < most:
             return b.as_strided(b.shape, (st[0], st[1], 1), b.storage_offset())
-        if b.shape[1] == 1:
+        if b.shape[1] == 1 and st[2] < most:
             return b.as_strided(b.shape, (st[0], 1, st[2]), b.storage_offset())
-    return b.contiguous()
+    return dense(b)
 
 
 def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:

@@ -25,6 +25,7 @@ import ctypes
 import torch
 
 from triturus_amd import _lib
+from triturus_amd.gmm import ROW_STRIDE_LIMIT, dense
 
 BLOCK = 32
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -59,9 +60,9 @@ def _check(q: MX4) -> None:
 def _unit(t: torch.Tensor) -> torch.Tensor:
     """Bytes of a row next to each other, in place where they are."""
     st = t.stride()
-    if (st[-1] == 1 or t.shape[-1] == 1) and min(st) >= 0:
+    if (st[-1] == 1 or t.shape[-1] == 1) and min(st) >= 0 and st[-2] < ROW_STRIDE_LIMIT:
         return t
-    return t.contiguous()
+    return dense(t)
 
 
 def _values(x: torch.Tensor) -> torch.Tensor:
@@ -134,7 +135,7 @@ def mm_mx4(a: torch.Tensor | MX4, b: MX4, sizes: torch.Tensor | None = None, *, 
         a_type = _type_code(a.dtype, "mm_mx4")
         if a.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("mm_mx4 has no gradient: detach its operand")
-        ac = as_ = _values(a)
+        ac = as_ = _values(a) if a.stride(0) < ROW_STRIDE_LIMIT else dense(a)
         dtype = dtype or a.dtype
         sa = _I64x2(ac.stride(0), 0)
     code = _type_code(dtype, "mm_mx4")
