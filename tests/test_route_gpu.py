@@ -262,3 +262,22 @@ def test_streams(dev):
             outs.append(route(x, 4))
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for o in outs for p, q in zip(o, want))
+
+
+def test_results_changed_in_place(dev):
+    """A result changed in place spoils nothing that autograd saved of the others."""
+    logits = torch.randn(70, 9, device=dev)
+    logits[3] = -math.inf
+    x, g = torch.randn(70, 8, device=dev, requires_grad=True), torch.randn(70, 2, device=dev)
+    want = route_grad(g, logits, route(logits, 2))
+    leaf = logits.clone().requires_grad_()
+    r = route(leaf, 2)
+    y = x[r.rows]
+    r.slots.clamp_(min=0), r.sizes.add_(1)
+    (r.weights * g).sum().backward()
+    assert torch.equal(leaf.grad, want)
+    r = route(logits, 2)
+    y = x[r.rows]
+    r.weights.mul_(2.5), r.experts.clamp_(min=0)
+    y.sum().backward()
+    assert torch.equal(x.grad.sum(1), 8.0 * torch.bincount(r.rows.long(), minlength=70))

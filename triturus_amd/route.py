@@ -29,6 +29,7 @@ from triturus_amd import _lib
 from triturus_amd.gmm import refuse_capture
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_empty = torch.empty_strided
 
 
 class Routes(NamedTuple):
@@ -56,10 +57,13 @@ def _route(logits: torch.Tensor, k: int, normalize: bool) -> Routes:
     code = _check(logits, k)
     T, E = logits.shape
     dev = logits.device
-    # one allocation for the four T x k results: they come and go together, and a small call is bound by the host
-    weights, experts, rows, slots = torch.empty((4, T, k), dtype=torch.int32, device=dev).unbind(0)
-    sizes = torch.empty(E, dtype=torch.int32, device=dev)
-    out = Routes(weights.view(torch.float32), experts, rows.view(-1), slots, sizes)
+    # five allocations: views of one would share its version, and a change of one in place would spoil what autograd saved of another
+    out = Routes(
+        _empty((T, k), (k, 1), dtype=torch.float32, device=dev), _empty((T, k), (k, 1), dtype=torch.int32, device=dev),
+        _empty((T * k,), (1,), dtype=torch.int32, device=dev), _empty((T, k), (k, 1), dtype=torch.int32, device=dev),
+        _empty((E,), (1,), dtype=torch.int32, device=dev),
+    )
+    weights, experts, rows, slots, sizes = out
     if T == 0:
         sizes.zero_()
         return out
