@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * WM *WN) void mx4_mm_kernel(Mx4Args g) {
 // 64 bytes of codes (4 blocks) by 64 columns: lane (n, g) takes block g of columns n, n + 16, .. and a column's 4 scale
 // bytes as one word.  A: the type of a's values, which the lane quantises itself on the way (32 neighbours of a
 // row: no other lane is needed, and a call is one launch), or uint8_t for codes.
-// FAST: at least 4 blocks in a row.
+// FAST: at least 4 blocks in a row.  One row, 4096 x 8192: 8.2 us (17.8 MB at 2.2 TB/s: one round of workgroups, bound by latency).
 template <typename A, int RT, bool FAST, int CW = 4, int W = 8, int D = 2>
 __global__ __launch_bounds__(64 * W) void mx4_few_kernel(Mx4Args g) {
     constexpr int COLS = 16 * CW;

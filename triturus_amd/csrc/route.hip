@@ -10,7 +10,8 @@
 // pair's place among the workgroup's is a population count of the bits below its row.  One workgroup does it all in one
 // launch; otherwise the first launch leaves the counts (a byte per expert and workgroup) and the last one adds up what
 // stands before it -- by itself up to kDirect workgroups, from a prefix sum made by a launch between them above that.
-// Bound: HBM for large T (logits once, 16 bytes a pair out), launches and latency for small.
+// Bound: launches and latency for small T (64 rows of 64: 3.3 us).  For large T the choice: 65536 rows of 128 fp32 logits take 8.5 us
+// (3.9 TB/s) and 1.2 to 1.4 more for each of the k choices, some 50 vector instructions; then 4.8 us for the sums, 7 for the places.
 #include "grouped.hpp"
 
 namespace trt {
