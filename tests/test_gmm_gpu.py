@@ -303,3 +303,34 @@ def test_rounds_of_the_largest_tile(dev, sizes, N, layout):
         s = torch.tensor(sizes, device=dev)
         close(_forward(a, b, s, 5), product64(a, b, sizes), product64(a.abs(), b.abs(), sizes), K)
     close(_weights(a, g, s, 5), weights64(a, g, sizes), weights64(a.abs(), g.abs(), sizes), max(sizes))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes,K,N", [([5000], 96, 200), ([4500, 0, 31, 2000], 130, 257), ([3000, 3000], 129, 64), ([0, 7000], 8, 8), ([9001], 1, 1)])
+def test_rows_cut_into_parts(dev, sizes, K, N, dtype):
+    """The matrices' gradient of few groups of many rows, with and without the workspace that the cut takes, and replayed."""
+    from triturus_amd import _lib
+    from triturus_amd.gmm import _weights
+
+    a, b, g = operands(dev, sum(sizes) + 3, len(sizes), K, N, dtype)
+    a[-3:], g[-3:] = math.nan, math.inf
+    s = torch.tensor(sizes, device=dev)
+    lib, code = _lib.load(), _lib.DTYPE_CODES[dtype]
+    T, E = a.shape[0], len(sizes)
+    want, size = weights64(a, g, sizes), weights64(a.abs(), g.abs(), sizes)
+    d = _weights(a, g, s)
+    assert lib.trt_gmm_weights_workspace_bytes(a.data_ptr(), g.data_ptr(), T, E, K, N, K, N, code, 0) >= 2 * E * 65536
+    close(d, want, size, max(sizes))
+    assert torch.equal(gmm_grad(g, a, b, s)[1], d)
+    plain = torch.full_like(d, math.nan)
+    assert lib.trt_gmm_weights(a.data_ptr(), g.data_ptr(), s.data_ptr(), plain.data_ptr(), T, E, K, N, K, N, code, 1, 0, None, 0,
+                               _lib.raw_stream(dev)) == 0
+    close(plain, want, size, max(sizes))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = _weights(a, g, s)
+    for _ in range(3):
+        captured.zero_()
+        eager = _weights(a, g, s)
+        graph.replay()
+        assert torch.equal(captured, d) and torch.equal(eager, d)

@@ -216,7 +216,21 @@ struct GmmArgs {
     int64_t M, N, K;      // rows: (unused), columns, contraction; weights: rows and columns of a matrix, (unused)
     int64_t ldx, ldy, y_group;  // strides in values; y_group: between the matrices (rows)
     uint32_t row_tiles, columns;  // weights: tiles of a matrix
+    uint32_t parts;               // weights: a group's rows are cut into this many, and `partial` takes their sums
+    float *partial;
 };
+
+// A part's sums in the order of the accumulators: 16 bytes a lane, [wavefront][i][j][q / 4][lane].
+template <int RT, int CT>
+__device__ __forceinline__ void store_partial(const floatx16 (&acc)[RT][CT], float *to, int wave) {
+    floatx4 *p = reinterpret_cast<floatx4 *>(to) + wave * (RT * CT * 4 * kWave) + lane_id();
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) p[((i * CT + j) * 4 + q) * kWave] = floatx4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+}
 
 // LDS of a tile: the stages, or the finished tile.
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN>
@@ -227,10 +241,10 @@ struct GmmLds {
     static constexpr int BYTES = kStages * STAGE > OUT ? kStages * STAGE : OUT;
 };
 
-// One tile: x, y and out at its first values, rows x cols of it exist, `terms` contracted values.
+// One tile: x, y and out at its first values, rows x cols of it exist, `terms` contracted values.  partial: not null for a part's sums.
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED>
 __device__ __forceinline__ void gmm_tile(const T *x, int64_t ldx, const T *y, int64_t ldy, T *out, int64_t N, int64_t rows, int64_t cols,
-                                         int64_t terms, char *lds) {
+                                         int64_t terms, char *lds, float *partial) {
     constexpr int THREADS = 64 * WM * WN, RT = BM / WM / 32, CT = BN / WN / 32;
     using X = Operand<T, XL, BM, THREADS>;
     using Y = Operand<T, YL, BN, THREADS>;
@@ -302,6 +316,7 @@ __device__ __forceinline__ void gmm_tile(const T *x, int64_t ldx, const T *y, in
             now = next, next = after, after = read;
         }
     }
+    if (XL == kOuter && partial) return store_partial(acc, partial, wave);
     store_tile<T, BM, BN, WM, WN>(acc, lds, wave, out, N, rows, cols);
 }
 
@@ -499,10 +514,11 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
     constexpr int STAGE = DIRECT ? 512 * kStepBytes : 16;
     __shared__ __attribute__((aligned(1024))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[STAGE];
     __shared__ __attribute__((aligned(16))) char lds[DIRECT ? 16 : GmmLds<T, XL, YL, BM, BN, WM, WN>::BYTES];
-    auto tile = [&](auto bm, auto bn, auto wm, auto wn, const T *x, const T *y, T *out, int64_t rows, int64_t cols, int64_t terms) {
+    auto tile = [&](auto bm, auto bn, auto wm, auto wn, const T *x, const T *y, T *out, int64_t rows, int64_t cols, int64_t terms,
+                    float *partial = nullptr) {
         constexpr int M = decltype(bm)::value, N = decltype(bn)::value, P = decltype(wm)::value, Q = decltype(wn)::value;
         if constexpr (DIRECT) gmm_direct_tile<T, XL, YL, M, N, P, Q>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, st0, st1, st2, st3);
-        else gmm_tile<T, XL, YL, M, N, P, Q, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, lds);
+        else gmm_tile<T, XL, YL, M, N, P, Q, ALIGNED>(x, g.ldx, y, g.ldy, out, g.N, rows, cols, terms, lds, partial);
     };
     constexpr std::integral_constant<int, BM> bm;
     constexpr std::integral_constant<int, BN> bn;
@@ -516,8 +532,9 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
         // group to group, so that matrices of few tiles fill all XCDs too.  (8 groups of 2048 rows on average, K = N = 4096: 1390 us
         // with a group per XCD, 680 us so.)
         const uint32_t per = g.row_tiles * g.columns, run = (per + kXcds - 1) / kXcds;
-        uint32_t e = blockIdx.x / kXcds / run;
-        const uint32_t in = (blockIdx.x + e) % kXcds * run + blockIdx.x / kXcds % run;
+        uint32_t e = blockIdx.x / kXcds / run, part = 0;
+        if (g.parts > 1) part = e % g.parts, e /= g.parts;
+        const uint32_t in = (blockIdx.x + e * g.parts + part) % kXcds * run + blockIdx.x / kXcds % run;
         if (in >= per) return;
         constexpr uint32_t kBand = 8;
         const uint32_t band = in / (kBand * g.columns), in_band = in - band * kBand * g.columns;
@@ -526,7 +543,14 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
         int64_t row0, terms;
         if (g.sizes.E <= kWave) e = group_by_length(g.sizes, e, row0, terms);  // long ones first: the last round is made of short ones
         else group_rows(g.sizes, e, row0, terms);
-        tile(bm, bn, wm, wn, x + row0 * g.ldx + m0, y + row0 * g.ldy + col0, out + (e * g.M + m0) * g.N + col0, g.M - m0, g.N - col0, terms);
+        float *partial = nullptr;
+        if (BM == 128 && g.parts > 1) {  // whole steps of every type but for the last part's end
+            const int64_t begin = terms * part / g.parts & ~(int64_t)31, end = part + 1 == g.parts ? terms : terms * (part + 1) / g.parts & ~(int64_t)31;
+            partial = g.partial + (((int64_t)part * g.sizes.E + e) * per + m0 / BM * g.columns + col0 / BN) * (BM * BN);
+            row0 += begin;
+            terms = end - begin;
+        }
+        tile(bm, bn, wm, wn, x + row0 * g.ldx + m0, y + row0 * g.ldy + col0, out + (e * g.M + m0) * g.N + col0, g.M - m0, g.N - col0, terms, partial);
     } else {
         GroupTile t;
         if (!find_tile<BM, CUT>(g.sizes, blockIdx.x, g.columns, t)) return;
@@ -553,6 +577,33 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
         }
         tile(bm, bn, wm, wn, x, y, out, t.rows, g.N - col0, terms);
     }
+}
+
+// The parts' sums of 128 x 128 tiles (2 x 2 wavefronts), added in order: a workgroup of one wavefront has 32 rows of a wavefront's 64 x 64.
+template <typename T>
+__global__ __launch_bounds__(kWave) void gmm_join_kernel(GmmArgs g) {
+    constexpr int RT = 2, CT = 2;
+    using Out = OutTile<T, 32, 32 * CT, 1, 1>;
+    __shared__ __attribute__((aligned(16))) char lds[Out::LDS];
+    const uint32_t per = g.row_tiles * g.columns, i = blockIdx.x % RT, wave = blockIdx.x / RT % 4, slot = blockIdx.x / (RT * 4), e = slot / per, in = slot % per;
+    const int64_t row0 = (int64_t)(in / g.columns) * 128 + wave / 2 * 64 + 32 * i, col0 = (int64_t)(in % g.columns) * 128 + wave % 2 * 64;
+    if (row0 >= g.M || col0 >= g.N) return;
+    const floatx4 *p = reinterpret_cast<const floatx4 *>(g.partial + (int64_t)slot * (128 * 128)) + (wave * RT + i) * (CT * 4 * kWave) + lane_id();
+    const int64_t stride = g.sizes.E * per * (int64_t)(128 * 128 / 4);
+    floatx4 sum[CT * 4];
+#pragma unroll
+    for (int q = 0; q < CT * 4; ++q) sum[q] = p[q * kWave];
+    for (uint32_t part = 1; part < g.parts; ++part) {
+        p += stride;
+#pragma unroll
+        for (int q = 0; q < CT * 4; ++q) sum[q] += p[q * kWave];
+    }
+    floatx16 acc[1][CT];
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[0][j][q] = sum[4 * j + q / 4][q % 4];
+    store_tile<T, 32, 32 * CT, 1, 1>(acc, lds, 0, static_cast<T *>(g.out) + ((int64_t)e * g.M + row0) * g.N + col0, g.N, g.M - row0, g.N - col0);
 }
 
 }  // namespace trt

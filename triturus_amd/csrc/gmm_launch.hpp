@@ -16,7 +16,8 @@ int launch_gmm_tile(GmmArgs g, int64_t E, int64_t T_rows, hipStream_t s) {
     int64_t blocks;
     if (XL == kOuter) {
         g.row_tiles = (uint32_t)ceil_div(g.M, BM);
-        blocks = E * ceil_div(g.row_tiles * (int64_t)g.columns, kXcds) * kXcds;
+        if (BM != 128 || !g.partial) g.parts = 1;
+        blocks = E * g.parts * ceil_div(g.row_tiles * (int64_t)g.columns, kXcds) * kXcds;
     } else {
         blocks = ceil_div(most_row_tiles(T_rows, E, BM) * (int64_t)g.columns, kXcds) * kXcds + (CUT ? kMostCut : 0);
     }
@@ -90,6 +91,31 @@ int choose_weights_tile(int64_t E, int64_t K, int64_t N) {
     const int64_t mid = E * ceil_div(K, 128) * ceil_div(N, 128), big = E * ceil_div(K, 256) * ceil_div(N, 256);
     if (mid < (sizeof(T) == 4 ? 1024 : 160)) return 2;
     return sizeof(T) == 2 && big >= 200 && big * 4 <= mid + mid / 7 ? 5 : 1;
+}
+
+// Into how many parts a group's rows are cut, on 128 x 128 tiles, where few groups of many rows have few tiles; 1: not.  `tile`: the
+// choice above.  The parts' sums are added in order by another launch.  Estimates in microseconds, fitted to 1..32 parts of 90 random
+// shapes: a step of 64 bytes a row with up to one, two or more workgroups on a CU, a launch and both ends of it, a part's tile
+// written and read, and how much longer the longest of several groups is than their mean.  The choice is 6 % behind the best number
+// on average, no cut 2.3 times (16384 rows, 512 x 512 of bf16: 175 us, 32 in parts; 2 groups, 1024 x 1024: 152 and 66).
+template <typename T>
+int64_t choose_weights_parts(int64_t T_rows, int64_t E, int64_t K, int64_t N, int tile) {
+    constexpr bool F32 = sizeof(T) == 4;
+    if (tile == 5) return 1;
+    const double steps = (double)ceil_div(ceil_div(T_rows, E) * (int64_t)sizeof(T), 64), mid = (double)(E * ceil_div(K, 128) * ceil_div(N, 128));
+    const double small = ceil((double)(E * ceil_div(K, 64) * ceil_div(N, 64)) / 256), longest = E > 1 ? 1.4 : 1.0, lone = E > 1 ? 1.65 : 1.0;
+    auto step = [](double workgroups) {
+        const double one = F32 ? 1.06 : 0.36, two = F32 ? 1.68 : 0.50, three = F32 ? 2.22 : 0.68;
+        return workgroups <= 256 ? one : workgroups <= 512 ? two : three * ceil(workgroups / 256) / 3;
+    };
+    const double least = F32 ? 0.364 : 0.314, shared = (F32 ? 0.21 : 0.122) * small;
+    double best = 0.95 * (3.7 + lone * steps * (tile == 2 ? (least > shared ? least : shared) : step(mid)));
+    int64_t parts = 1;
+    for (int64_t p = 2; p <= 32 && (double)p * 4 <= steps; ++p) {
+        const double us = (F32 ? 14.5 : 12.8) + longest * steps / (double)p * step(mid * (double)p) + (double)p * mid * 0.02;
+        if (us < best) best = us, parts = p;
+    }
+    return parts;
 }
 
 // ---- operands off the 16-byte boundaries -------------------------------------------------------------------------------
@@ -173,8 +199,12 @@ struct Workspace {
 template <typename T, int XL, int YL>
 int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &w, hipStream_t s) {
     double us = 0.0;
+    g.parts = 1;
     if constexpr (XL == kOuter) {
-        if (tile == 0) tile = choose_weights_tile<T>(E, g.M, g.N);
+        if (tile == 0) {
+            tile = choose_weights_tile<T>(E, g.M, g.N);
+            g.parts = (uint32_t)choose_weights_parts<T>(T_rows, E, g.M, g.N, tile);
+        }
         us = 10.0 + 2.0 * (double)T_rows * (double)g.M * (double)g.N / (sizeof(T) == 4 ? 60e6 : 900e6);
     } else {
         const int best = choose_gmm_tile<T>(T_rows, E, g.N, g.K, YL == kInner, &us);
@@ -183,12 +213,15 @@ int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &
     // few rows are bound by reading the matrices, and a copy reads and writes them
     const bool few = XL == kInner && tile >= 2 && tile <= 4;
     const PadPlan pads = few ? PadPlan{false, false, 0} : plan_pads<T, XL, YL>(g, E, T_rows, us, XL == kOuter ? 1.2 : YL == kOuter ? 0.8 : 0.5);
+    const size_t partial = g.parts > 1 ? (size_t)(g.parts * E * ceil_div(g.M, 128) * ceil_div(g.N, 128)) * (128 * 128 * sizeof(float)) : 0;
     if (w.query) {
-        *w.query = pads.bytes;
+        *w.query = pads.bytes + partial;
         return TRT_OK;
     }
+    const bool work = w.p && w.bytes >= pads.bytes + partial;  // without a workspace operands are read as they are, and rows not cut
+    if (work && partial) g.partial = reinterpret_cast<float *>(static_cast<char *>(w.p) + pads.bytes), tile = 1;
     bool aligned = chunks_aligned<T>(g.x, {g.ldx, XL == kInner ? g.K : g.M}) && chunks_aligned<T>(g.y, {g.ldy, g.y_group, YL == kInner ? g.K : g.N});
-    if (pads.bytes && w.p && w.bytes >= pads.bytes) {  // without a workspace the operands are read as they are
+    if (pads.bytes && work) {
         const int status = apply_pads<T, XL, YL>(g, E, T_rows, pads, w.p, s);
         if (status) return status;
         aligned = true;
@@ -213,8 +246,17 @@ int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &
             return aligned ? launch_gmm_tile<T, XL, YL, 64, 64, 2, 2, true>(g, E, T_rows, s)
                            : launch_gmm_tile<T, XL, YL, 64, 64, 2, 2, false>(g, E, T_rows, s);
     }
-    return aligned ? launch_gmm_tile<T, XL, YL, 128, 128, 2, 2, true>(g, E, T_rows, s)
-                   : launch_gmm_tile<T, XL, YL, 128, 128, 2, 2, false>(g, E, T_rows, s);
+    const int status = aligned ? launch_gmm_tile<T, XL, YL, 128, 128, 2, 2, true>(g, E, T_rows, s)
+                               : launch_gmm_tile<T, XL, YL, 128, 128, 2, 2, false>(g, E, T_rows, s);
+    if constexpr (XL == kOuter) {
+        if (!status && g.partial) {
+            g.row_tiles = (uint32_t)ceil_div(g.M, 128), g.columns = (uint32_t)ceil_div(g.N, 128);
+            const int64_t blocks = E * g.row_tiles * g.columns * 8;
+            hipLaunchKernelGGL(gmm_join_kernel<T>, dim3((unsigned)blocks), dim3(kWave), 0, s, g);
+            return (int)hipGetLastError();
+        }
+    }
+    return status;
 }
 
 template <typename T>

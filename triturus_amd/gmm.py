@@ -69,6 +69,11 @@ def _matrices(b: torch.Tensor) -> torch.Tensor:
     return dense(b)
 
 
+def _few_tiles(T: int, E: int, K: int, N: int) -> bool:
+    """Whether the library may cut the rows of the matrices' gradient, which takes a workspace."""
+    return E * K * N <= 1 << 23 and T >= 128 * E
+
+
 def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:
     sa, sb, ss = a.shape, b.shape, sizes.shape
     assert len(sa) == 2 and len(sb) == 3 and len(ss) == 1
@@ -123,7 +128,7 @@ def _weights(a: torch.Tensor, g: torch.Tensor, sizes: torch.Tensor, tile: int = 
     lib, code = _lib.load(), _lib.DTYPE_CODES[dtype]
     pa, pg, lda, ldg = a.data_ptr(), g.data_ptr(), a.stride(0), g.stride(0)
     ws_ptr, nbytes, ws = None, 0, None
-    if (pa | pg) & 15 or (K | N | lda | ldg) & 7:  # then a copy may pay
+    if (pa | pg) & 15 or (K | N | lda | ldg) & 7 or _few_tiles(T, E, K, N):  # a copy or a cut may pay
         nbytes = lib.trt_gmm_weights_workspace_bytes(pa, pg, T, E, K, N, lda, ldg, code, tile)
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -178,7 +183,7 @@ def gmm_grad(g: torch.Tensor, a: torch.Tensor, b: torch.Tensor, sizes: torch.Ten
     lib, code = _lib.load(), _lib.DTYPE_CODES[a.dtype]
     pg, pa, pb, ldg, lda, sb = g.data_ptr(), a.data_ptr(), b.data_ptr(), g.stride(0), a.stride(0), _lib.strides3(b)
     ws_ptr, nbytes, ws = None, 0, None
-    if (pg | pa | pb) & 15 or (K | N | ldg | lda | sb[0] | (sb[2] if sb[1] == 1 else sb[1])) & 7:  # then a copy may pay
+    if (pg | pa | pb) & 15 or (K | N | ldg | lda | sb[0] | (sb[2] if sb[1] == 1 else sb[1])) & 7 or _few_tiles(T, E, K, N):  # a copy or a cut may pay
         nbytes = lib.trt_gmm_grad_workspace_bytes(pg, pa, pb, T, E, K, N, ldg, lda, sb, code)
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
