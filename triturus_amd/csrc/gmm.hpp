@@ -590,13 +590,18 @@ __global__ __launch_bounds__(kWave) void gmm_join_kernel(GmmArgs g) {
     if (row0 >= g.M || col0 >= g.N) return;
     const floatx4 *p = reinterpret_cast<const floatx4 *>(g.partial + (int64_t)slot * (128 * 128)) + (wave * RT + i) * (CT * 4 * kWave) + lane_id();
     const int64_t stride = g.sizes.E * per * (int64_t)(128 * 128 / 4);
-    floatx4 sum[CT * 4];
+    floatx4 sum[CT * 4] = {};
+    constexpr uint32_t AHEAD = 4;  // parts whose loads are on their way at once
+    for (uint32_t part = 0; part < g.parts; part += AHEAD, p += AHEAD * stride) {
+        floatx4 v[AHEAD][CT * 4];
 #pragma unroll
-    for (int q = 0; q < CT * 4; ++q) sum[q] = p[q * kWave];
-    for (uint32_t part = 1; part < g.parts; ++part) {
-        p += stride;
+        for (uint32_t a = 0; a < AHEAD; ++a)
 #pragma unroll
-        for (int q = 0; q < CT * 4; ++q) sum[q] += p[q * kWave];
+            for (int q = 0; q < CT * 4; ++q) v[a][q] = part + a < g.parts ? p[a * stride + q * kWave] : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t a = 0; a < AHEAD; ++a)
+#pragma unroll
+            for (int q = 0; q < CT * 4; ++q) sum[q] += v[a][q];
     }
     floatx16 acc[1][CT];
 #pragma unroll

@@ -96,23 +96,23 @@ int choose_weights_tile(int64_t E, int64_t K, int64_t N) {
 // Into how many parts a group's rows are cut, on 128 x 128 tiles, where few groups of many rows have few tiles; 1: not.  `tile`: the
 // choice above.  The parts' sums are added in order by another launch.  Estimates in microseconds, fitted to 1..32 parts of 90 random
 // shapes: a step of 64 bytes a row with up to one, two or more workgroups on a CU, a launch and both ends of it, a part's tile
-// written and read, and how much longer the longest of several groups is than their mean.  The choice is 6 % behind the best number
-// on average, no cut 2.3 times (16384 rows, 512 x 512 of bf16: 175 us, 32 in parts; 2 groups, 1024 x 1024: 152 and 66).
+// written and read, and how much longer the longest of several groups is than their mean.  The choice is 4 % behind the best number
+// on average, no cut 2.4 times (16384 rows, 512 x 512 of bf16: 175 us, 28 in parts; 2 groups, 1024 x 1024: 152 and 67).
 template <typename T>
 int64_t choose_weights_parts(int64_t T_rows, int64_t E, int64_t K, int64_t N, int tile) {
     constexpr bool F32 = sizeof(T) == 4;
     if (tile == 5) return 1;
     const double steps = (double)ceil_div(ceil_div(T_rows, E) * (int64_t)sizeof(T), 64), mid = (double)(E * ceil_div(K, 128) * ceil_div(N, 128));
-    const double small = ceil((double)(E * ceil_div(K, 64) * ceil_div(N, 64)) / 256), longest = E > 1 ? 1.4 : 1.0, lone = E > 1 ? 1.65 : 1.0;
+    const double small = ceil((double)(E * ceil_div(K, 64) * ceil_div(N, 64)) / 256), longest = E > 1 ? 1.45 : 1.0, lone = E > 1 ? 1.65 : 1.0;
     auto step = [](double workgroups) {
-        const double one = F32 ? 1.06 : 0.36, two = F32 ? 1.68 : 0.50, three = F32 ? 2.22 : 0.68;
+        const double one = F32 ? 1.06 : 0.36, two = F32 ? 1.66 : 0.48, three = F32 ? 2.20 : 0.665;
         return workgroups <= 256 ? one : workgroups <= 512 ? two : three * ceil(workgroups / 256) / 3;
     };
     const double least = F32 ? 0.364 : 0.314, shared = (F32 ? 0.21 : 0.122) * small;
-    double best = 0.95 * (3.7 + lone * steps * (tile == 2 ? (least > shared ? least : shared) : step(mid)));
+    double best = 0.97 * (3.7 + lone * steps * (tile == 2 ? (least > shared ? least : shared) : step(mid)));
     int64_t parts = 1;
     for (int64_t p = 2; p <= 32 && (double)p * 4 <= steps; ++p) {
-        const double us = (F32 ? 14.5 : 12.8) + longest * steps / (double)p * step(mid * (double)p) + (double)p * mid * 0.02;
+        const double us = (F32 ? 13.9 : 11.1) + longest * steps / (double)p * step(mid * (double)p) + (double)p * mid * 0.019;
         if (us < best) best = us, parts = p;
     }
     return parts;
