@@ -216,11 +216,11 @@ struct GmmArgs {
     int64_t M, N, K;      // rows: (unused), columns, contraction; weights: rows and columns of a matrix, (unused)
     int64_t ldx, ldy, y_group;  // strides in values; y_group: between the matrices (rows)
     uint32_t row_tiles, columns;  // weights: tiles of a matrix
-    uint32_t parts;               // weights: a group's rows are cut into this many, and `partial` takes their sums
+    Divider piece;                // weights: rows of a piece, whose sums go to `partial`; d = 0: groups are whole
     float *partial;
 };
 
-// A part's sums in the order of the accumulators: 16 bytes a lane, [wavefront][i][j][q / 4][lane].
+// A piece's sums in the order of the accumulators: 16 bytes a lane, [wavefront][i][j][q / 4][lane].
 template <int RT, int CT>
 __device__ __forceinline__ void store_partial(const floatx16 (&acc)[RT][CT], float *to, int wave) {
     floatx4 *p = reinterpret_cast<floatx4 *>(to) + wave * (RT * CT * 4 * kWave) + lane_id();
@@ -241,7 +241,7 @@ struct GmmLds {
     static constexpr int BYTES = kStages * STAGE > OUT ? kStages * STAGE : OUT;
 };
 
-// One tile: x, y and out at its first values, rows x cols of it exist, `terms` contracted values.  partial: not null for a part's sums.
+// One tile: x, y and out at its first values, rows x cols of it exist, `terms` contracted values.  partial: not null for a piece's sums.
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED>
 __device__ __forceinline__ void gmm_tile(const T *x, int64_t ldx, const T *y, int64_t ldy, T *out, int64_t N, int64_t rows, int64_t cols,
                                          int64_t terms, char *lds, float *partial) {
@@ -532,24 +532,23 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
         // group to group, so that matrices of few tiles fill all XCDs too.  (8 groups of 2048 rows on average, K = N = 4096: 1390 us
         // with a group per XCD, 680 us so.)
         const uint32_t per = g.row_tiles * g.columns, run = (per + kXcds - 1) / kXcds;
-        uint32_t e = blockIdx.x / kXcds / run, part = 0;
-        if (g.parts > 1) part = e % g.parts, e /= g.parts;
-        const uint32_t in = (blockIdx.x + e * g.parts + part) % kXcds * run + blockIdx.x / kXcds % run;
+        uint32_t e = blockIdx.x / kXcds / run;  // or the piece's number
+        const uint32_t in = (blockIdx.x + e) % kXcds * run + blockIdx.x / kXcds % run;
         if (in >= per) return;
         constexpr uint32_t kBand = 8;
         const uint32_t band = in / (kBand * g.columns), in_band = in - band * kBand * g.columns;
         const uint32_t high = g.row_tiles - band * kBand < kBand ? g.row_tiles - band * kBand : kBand;
         const int64_t m0 = (int64_t)(band * kBand + in_band % high) * BM, col0 = (int64_t)(in_band / high) * BN;
         int64_t row0, terms;
-        if (g.sizes.E <= kWave) e = group_by_length(g.sizes, e, row0, terms);  // long ones first: the last round is made of short ones
-        else group_rows(g.sizes, e, row0, terms);
         float *partial = nullptr;
-        if (BM == 128 && g.parts > 1) {  // whole steps of every type but for the last part's end
-            const int64_t begin = terms * part / g.parts & ~(int64_t)31, end = part + 1 == g.parts ? terms : terms * (part + 1) / g.parts & ~(int64_t)31;
-            partial = g.partial + (((int64_t)part * g.sizes.E + e) * per + m0 / BM * g.columns + col0 / BN) * (BM * BN);
-            row0 += begin;
-            terms = end - begin;
-        }
+        if (BM == 128 && g.piece.d) {
+            GroupPieces p;
+            if (!find_pieces(g.sizes, g.piece, p, [&](uint32_t, uint32_t first, uint32_t count) { return e < first + count; })) return;
+            partial = g.partial + ((int64_t)e * per + m0 / BM * g.columns + col0 / BN) * (BM * BN);
+            row0 = p.start + (int64_t)(e - p.first) * g.piece.d;
+            terms = p.end - row0 < g.piece.d ? p.end - row0 : g.piece.d;
+        } else if (g.sizes.E <= kWave) e = group_by_length(g.sizes, e, row0, terms);  // long ones first: the last round is made of short ones
+        else group_rows(g.sizes, e, row0, terms);
         tile(bm, bn, wm, wn, x + row0 * g.ldx + m0, y + row0 * g.ldy + col0, out + (e * g.M + m0) * g.N + col0, g.M - m0, g.N - col0, terms, partial);
     } else {
         GroupTile t;
@@ -579,25 +578,27 @@ __global__ __launch_bounds__(64 * WM *WN) void gmm_kernel(GmmArgs g) {
     }
 }
 
-// The parts' sums of 128 x 128 tiles (2 x 2 wavefronts), added in order: a workgroup of one wavefront has 32 rows of a wavefront's 64 x 64.
+// The pieces' sums of 128 x 128 tiles (2 x 2 wavefronts), added in order: a workgroup of one wavefront has 32 rows of a wavefront's 64 x 64.
 template <typename T>
 __global__ __launch_bounds__(kWave) void gmm_join_kernel(GmmArgs g) {
     constexpr int RT = 2, CT = 2;
     using Out = OutTile<T, 32, 32 * CT, 1, 1>;
     __shared__ __attribute__((aligned(16))) char lds[Out::LDS];
-    const uint32_t per = g.row_tiles * g.columns, i = blockIdx.x % RT, wave = blockIdx.x / RT % 4, slot = blockIdx.x / (RT * 4), e = slot / per, in = slot % per;
+    const uint32_t per = g.row_tiles * g.columns, i = blockIdx.x % RT, wave = blockIdx.x / RT % 4, in = blockIdx.x / (RT * 4) % per, e = blockIdx.x / (RT * 4) / per;
     const int64_t row0 = (int64_t)(in / g.columns) * 128 + wave / 2 * 64 + 32 * i, col0 = (int64_t)(in % g.columns) * 128 + wave % 2 * 64;
     if (row0 >= g.M || col0 >= g.N) return;
-    const floatx4 *p = reinterpret_cast<const floatx4 *>(g.partial + (int64_t)slot * (128 * 128)) + (wave * RT + i) * (CT * 4 * kWave) + lane_id();
-    const int64_t stride = g.sizes.E * per * (int64_t)(128 * 128 / 4);
+    GroupPieces own;
+    if (!find_pieces(g.sizes, g.piece, own, [&](uint32_t group, uint32_t, uint32_t) { return group == e; })) return;
+    const floatx4 *p = reinterpret_cast<const floatx4 *>(g.partial + ((int64_t)own.first * per + in) * (128 * 128)) + (wave * RT + i) * (CT * 4 * kWave) + lane_id();
+    const int64_t stride = per * (int64_t)(128 * 128 / 4);
     floatx4 sum[CT * 4] = {};
-    constexpr uint32_t AHEAD = 4;  // parts whose loads are on their way at once
-    for (uint32_t part = 0; part < g.parts; part += AHEAD, p += AHEAD * stride) {
+    constexpr uint32_t AHEAD = 4;  // pieces whose loads are on their way at once
+    for (uint32_t piece = 0; piece < own.count; piece += AHEAD, p += AHEAD * stride) {
         floatx4 v[AHEAD][CT * 4];
 #pragma unroll
         for (uint32_t a = 0; a < AHEAD; ++a)
 #pragma unroll
-            for (int q = 0; q < CT * 4; ++q) v[a][q] = part + a < g.parts ? p[a * stride + q * kWave] : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int q = 0; q < CT * 4; ++q) v[a][q] = piece + a < own.count ? p[a * stride + q * kWave] : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t a = 0; a < AHEAD; ++a)
 #pragma unroll

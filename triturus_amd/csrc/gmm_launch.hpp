@@ -8,6 +8,8 @@
 
 namespace trt {
 
+inline int64_t most_pieces(int64_t T, int64_t E, int64_t len) { return T / len + (E < T ? E : T); }
+
 // Tiles of the rows' products: 1 = 128 x 128, 2, 3, 4 = 16, 32, 64 rows x 64 columns of the few-row kernel, 5 = 256 x 256
 // (16-bit types) or 64 x 64 (fp32).  Of the weights' gradient: 1 = 128 x 128, 2 = 64 x 64, 5 = 256 x 256.
 template <typename T, int XL, int YL, int BM, int BN, int WM, int WN, bool ALIGNED, bool CUT = false>
@@ -16,8 +18,9 @@ int launch_gmm_tile(GmmArgs g, int64_t E, int64_t T_rows, hipStream_t s) {
     int64_t blocks;
     if (XL == kOuter) {
         g.row_tiles = (uint32_t)ceil_div(g.M, BM);
-        if (BM != 128 || !g.partial) g.parts = 1;
-        blocks = E * g.parts * ceil_div(g.row_tiles * (int64_t)g.columns, kXcds) * kXcds;
+        const bool cut = BM == 128 && g.partial;
+        if (!cut) g.piece = {};
+        blocks = (cut ? most_pieces(T_rows, E, g.piece.d) : E) * ceil_div(g.row_tiles * (int64_t)g.columns, kXcds) * kXcds;
     } else {
         blocks = ceil_div(most_row_tiles(T_rows, E, BM) * (int64_t)g.columns, kXcds) * kXcds + (CUT ? kMostCut : 0);
     }
@@ -93,29 +96,34 @@ int choose_weights_tile(int64_t E, int64_t K, int64_t N) {
     return sizeof(T) == 2 && big >= 200 && big * 4 <= mid + mid / 7 ? 5 : 1;
 }
 
-// Into how many parts a group's rows are cut, on 128 x 128 tiles, where few groups of many rows have few tiles; 1: not.  `tile`: the
-// choice above.  The parts' sums are added in order by another launch.  Estimates in microseconds, fitted to 1..32 parts of 90 random
-// shapes: a step of 64 bytes a row with up to one, two or more workgroups on a CU, a launch and both ends of it, a part's tile
-// written and read, and how much longer the longest of several groups is than their mean.  The choice is 4 % behind the best number
-// on average, no cut 2.4 times (16384 rows, 512 x 512 of bf16: 175 us, 28 in parts; 2 groups, 1024 x 1024: 152 and 67).
+// Into pieces of how many rows the groups are cut, on 128 x 128 tiles, where few tiles have long contractions; 0: not.  `tile`: the
+// choice above.  The pieces' sums are added in order by another launch.  Estimates in microseconds, fitted to pieces of a
+// 1/32 .. 1 of the mean group on 90 random shapes: a step of 64 bytes a row with up to one, two or more workgroups on a CU, both
+// launches, a piece's tile written and read, and without pieces how much longer the longest of several groups is than their mean.
+// The choice is 6 to 7 % behind the best pieces on average, none 2.3 times (16384 rows, 512 x 512 of bf16: 175 us, 29 in pieces;
+// 16 uneven groups, 256 x 512: 48 and 26).
 template <typename T>
-int64_t choose_weights_parts(int64_t T_rows, int64_t E, int64_t K, int64_t N, int tile) {
+int64_t choose_weights_piece(int64_t T_rows, int64_t E, int64_t K, int64_t N, int tile) {
     constexpr bool F32 = sizeof(T) == 4;
-    if (tile == 5) return 1;
-    const double steps = (double)ceil_div(ceil_div(T_rows, E) * (int64_t)sizeof(T), 64), mid = (double)(E * ceil_div(K, 128) * ceil_div(N, 128));
-    const double small = ceil((double)(E * ceil_div(K, 64) * ceil_div(N, 64)) / 256), longest = E > 1 ? 1.45 : 1.0, lone = E > 1 ? 1.65 : 1.0;
+    if (tile == 5) return 0;
+    const double matrix = (double)(ceil_div(K, 128) * ceil_div(N, 128)), mid = (double)E * matrix;
+    const double small = ceil((double)(E * ceil_div(K, 64) * ceil_div(N, 64)) / 256), longest = 1.0 + (F32 ? 0.26 : 0.50) * log2((double)(E < 16 ? E : 16));
     auto step = [](double workgroups) {
-        const double one = F32 ? 1.06 : 0.36, two = F32 ? 1.66 : 0.48, three = F32 ? 2.20 : 0.665;
+        const double one = F32 ? 1.05 : 0.36, two = F32 ? 1.93 : 0.57, three = F32 ? 2.79 : 0.855;
         return workgroups <= 256 ? one : workgroups <= 512 ? two : three * ceil(workgroups / 256) / 3;
     };
-    const double least = F32 ? 0.364 : 0.314, shared = (F32 ? 0.21 : 0.122) * small;
-    double best = 0.97 * (3.7 + lone * steps * (tile == 2 ? (least > shared ? least : shared) : step(mid)));
-    int64_t parts = 1;
-    for (int64_t p = 2; p <= 32 && (double)p * 4 <= steps; ++p) {
-        const double us = (F32 ? 13.9 : 11.1) + longest * steps / (double)p * step(mid * (double)p) + (double)p * mid * 0.019;
-        if (us < best) best = us, parts = p;
+    const double steps = (double)ceil_div(ceil_div(T_rows, E) * (int64_t)sizeof(T), 64);
+    const double least = F32 ? 0.382 : 0.314, shared = (F32 ? 0.22 : 0.122) * small;
+    double best = 0.97 * (3.3 + longest * steps * (tile == 2 ? (least > shared ? least : shared) : step(mid)));
+    int64_t rows = 0;
+    for (int64_t p = 1; p <= 32; ++p) {
+        const int64_t len = ceil_div(ceil_div(T_rows, E * p), 32) * 32;
+        if (len * (int64_t)sizeof(T) < 4 * 64) break;
+        const double n = E == 1 ? (double)ceil_div(T_rows, len) : (double)(T_rows / len) + 0.5 * (double)E, w = n * matrix;
+        const double us = (F32 ? 13.3 : 11.5) + (double)(len * (int64_t)sizeof(T) / 64) * step(w) + w * 0.021;
+        if (us < best) best = us, rows = len;
     }
-    return parts;
+    return rows;
 }
 
 // ---- operands off the 16-byte boundaries -------------------------------------------------------------------------------
@@ -199,11 +207,11 @@ struct Workspace {
 template <typename T, int XL, int YL>
 int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &w, hipStream_t s) {
     double us = 0.0;
-    g.parts = 1;
+    int64_t piece = 0;
     if constexpr (XL == kOuter) {
         if (tile == 0) {
             tile = choose_weights_tile<T>(E, g.M, g.N);
-            g.parts = (uint32_t)choose_weights_parts<T>(T_rows, E, g.M, g.N, tile);
+            piece = choose_weights_piece<T>(T_rows, E, g.M, g.N, tile);
         }
         us = 10.0 + 2.0 * (double)T_rows * (double)g.M * (double)g.N / (sizeof(T) == 4 ? 60e6 : 900e6);
     } else {
@@ -213,13 +221,13 @@ int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &
     // few rows are bound by reading the matrices, and a copy reads and writes them
     const bool few = XL == kInner && tile >= 2 && tile <= 4;
     const PadPlan pads = few ? PadPlan{false, false, 0} : plan_pads<T, XL, YL>(g, E, T_rows, us, XL == kOuter ? 1.2 : YL == kOuter ? 0.8 : 0.5);
-    const size_t partial = g.parts > 1 ? (size_t)(g.parts * E * ceil_div(g.M, 128) * ceil_div(g.N, 128)) * (128 * 128 * sizeof(float)) : 0;
+    const size_t partial = piece ? (size_t)(most_pieces(T_rows, E, piece) * ceil_div(g.M, 128) * ceil_div(g.N, 128)) * (128 * 128 * sizeof(float)) : 0;
     if (w.query) {
         *w.query = pads.bytes + partial;
         return TRT_OK;
     }
     const bool work = w.p && w.bytes >= pads.bytes + partial;  // without a workspace operands are read as they are, and rows not cut
-    if (work && partial) g.partial = reinterpret_cast<float *>(static_cast<char *>(w.p) + pads.bytes), tile = 1;
+    if (work && partial) g.partial = reinterpret_cast<float *>(static_cast<char *>(w.p) + pads.bytes), g.piece = divider((uint32_t)piece), tile = 1;
     bool aligned = chunks_aligned<T>(g.x, {g.ldx, XL == kInner ? g.K : g.M}) && chunks_aligned<T>(g.y, {g.ldy, g.y_group, YL == kInner ? g.K : g.N});
     if (pads.bytes && work) {
         const int status = apply_pads<T, XL, YL>(g, E, T_rows, pads, w.p, s);

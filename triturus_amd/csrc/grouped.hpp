@@ -172,6 +172,29 @@ inline Divider divider(uint32_t d) {
 }
 __device__ __forceinline__ uint32_t divide(uint32_t n, const Divider &v) { return (__umulhi(n, v.m) + n) >> v.s; }
 
+// Groups cut into pieces of len.d rows, the last one of a group shorter, numbered through all groups.  The first lane `want(first,
+// count)` holds for, over all groups' first pieces and their numbers of pieces, says which group it is; rows [start, end) are its own.
+struct GroupPieces {
+    uint32_t group, first, count, start, end;
+};
+template <typename F>
+__device__ __forceinline__ bool find_pieces(const Sizes &s, const Divider &len, GroupPieces &p, F want) {
+    uint32_t before = 0, start = 0, end = 0, pieces = 0;
+    for (uint32_t e = 0; e < s.E; e += kWave) {
+        chunk_rows(s, e, before, start, end);
+        const bool there = e + lane_id() < s.E;
+        const uint32_t n = there ? end - start : 0, count = n ? divide(n - 1, len) + 1 : 0, incl = wave_prefix(count);
+        const uint64_t mask = __ballot(there && want(e + lane_id(), pieces + incl - count, count));
+        if (mask) {
+            const int who = __builtin_ctzll(mask);
+            p = {e + who, lane_value(pieces + incl - count, who), lane_value(count, who), lane_value(start, who), lane_value(end, who)};
+            return true;
+        }
+        pieces += lane_value(incl, kWave - 1);
+    }
+    return false;
+}
+
 // ---- 16 bytes of a row -----------------------------------------------------------------------------
 // `left` elements of the row remain from p on (<= 0: none).  A full chunk is one load, whatever the
 // alignment (global memory takes 16-byte loads from any address); an end of a row that is not a whole
