@@ -332,7 +332,7 @@ int trt_gmm_weights(const void *a, const void *g, const void *sizes, void *d, in
 size_t trt_gmm_weights_workspace_bytes(const void *a, const void *g, int64_t T, int64_t E, int64_t K, int64_t N,
                                        int64_t lda, int64_t ldg, int dtype, int tile);
 /* Both gradients of sum(g * c) in one call: da (T x K) as trt_gmm with b's last two axes exchanged, db (E x K x N) as trt_gmm_weights;
- * the workspace serves one after the other. */
+ * an operand of both is copied once. */
 int trt_gmm_grad(const void *g, const void *a, const void *b, const void *sizes, void *da, void *db, int64_t T, int64_t E,
                  int64_t K, int64_t N, int64_t ldg, int64_t lda, const int64_t sb[3], int dtype, int wide_sizes,
                  void *workspace, size_t workspace_bytes, void *stream);

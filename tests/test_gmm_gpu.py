@@ -336,3 +336,23 @@ def test_rows_cut_into_pieces(dev, sizes, K, N, dtype):
         eager = _weights(a, g, s)
         graph.replay()
         assert torch.equal(captured, d) and torch.equal(eager, d)
+
+
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("K,N", [(257, 130), (256, 131), (259, 128)])
+def test_gradients_with_and_without_copies(dev, K, N, layout):
+    """Operands off the boundaries, all or one of them: copied once for both products, or read as they lie without a workspace."""
+    from triturus_amd import _lib
+
+    sizes, dtype = [500, 0, 700, 3], torch.float16
+    a, b, g = operands(dev, sum(sizes) + 2, len(sizes), K, N, dtype, layout)
+    s, bt = torch.tensor(sizes, device=dev, dtype=torch.int32), b.transpose(1, 2)
+    lib, code, T, E = _lib.load(), _lib.DTYPE_CODES[dtype], a.shape[0], len(sizes)
+    args = g.data_ptr(), a.data_ptr(), b.data_ptr()
+    assert lib.trt_gmm_grad_workspace_bytes(*args, T, E, K, N, N, K, _lib.strides3(b), code) > 0
+    da, db = torch.full_like(a, math.nan), torch.full((E, K, N), math.nan, dtype=dtype, device=dev)
+    assert lib.trt_gmm_grad(*args, s.data_ptr(), da.data_ptr(), db.data_ptr(), T, E, K, N, N, K, _lib.strides3(b), code, 0, None, 0,
+                            _lib.raw_stream(dev)) == 0
+    for got in ((da, db), gmm_grad(g, a, b, s)):
+        close(got[0], product64(g, bt, sizes), product64(g.abs(), bt.abs(), sizes), N)
+        close(got[1], weights64(a, g, sizes), weights64(a.abs(), g.abs(), sizes), max(sizes))

@@ -19,39 +19,75 @@ int dispatch(const GmmArgs &g, int64_t E, int64_t T, bool weights, bool y_inner,
     }
 }
 
-int rows_product(const void *a, const void *b, const void *sizes, void *c, int64_t T, int64_t E, int64_t K, int64_t N, int64_t lda,
-                 const int64_t sb[3], int dtype, int wide_sizes, int tile, const Workspace &w, void *stream) {
+// `query`: only the workspace is asked for, without sizes and result.
+int rows_args(const void *a, const void *b, const void *sizes, void *c, int64_t T, int64_t E, int64_t K, int64_t N, int64_t lda,
+              const int64_t sb[3], int dtype, int wide_sizes, int tile, const void *workspace, bool query, GmmArgs &g, bool &inner) {
     const size_t size = type_size(dtype);
     if (!a || !b || !sb || T <= 0 || E <= 0 || K <= 0 || N <= 0 || !size || tile < 0 || tile > TRT_GMM_TILES) return TRT_E_INVALID;
-    if (!w.query && (!sizes || !c)) return TRT_E_INVALID;
-    if (lda < 0 || sb[0] < 0 || sb[1] < 0 || sb[2] < 0 || (reinterpret_cast<uintptr_t>(w.p) & 15)) return TRT_E_LAYOUT;
-    const bool inner = sb[1] == 1;
+    if (!query && (!sizes || !c)) return TRT_E_INVALID;
+    if (lda < 0 || sb[0] < 0 || sb[1] < 0 || sb[2] < 0 || (reinterpret_cast<uintptr_t>(workspace) & 15)) return TRT_E_LAYOUT;
+    inner = sb[1] == 1;
     if (!inner && sb[2] != 1) return TRT_E_LAYOUT;
     const int64_t ldb = inner ? sb[2] : sb[1];
     if (!stride_fits(lda, size) || !stride_fits(ldb, size) || !stride_fits(N, size) || !stride_fits(K, size) || T >= (int64_t)1 << 31 ||
         E >= (int64_t)1 << 31)
         return TRT_E_RANGE;
-    GmmArgs g = {};
+    g = {};
     g.x = a, g.y = b, g.out = c;
     g.sizes = {sizes, wide_sizes, E, T};
     g.N = N, g.K = K, g.ldx = lda, g.ldy = ldb, g.y_group = sb[0];
-    return dispatch(g, E, T, false, inner, dtype, tile, w, stream);
+    return TRT_OK;
+}
+
+int weights_args(const void *a, const void *g_, const void *sizes, void *d, int64_t T, int64_t E, int64_t K, int64_t N, int64_t lda,
+                 int64_t ldg, int dtype, int wide_sizes, int tile, const void *workspace, bool query, GmmArgs &g) {
+    const size_t size = type_size(dtype);
+    if (!a || !g_ || T <= 0 || E <= 0 || K <= 0 || N <= 0 || !size || tile < 0 || tile > TRT_GMM_TILES) return TRT_E_INVALID;
+    if (!query && (!sizes || !d)) return TRT_E_INVALID;
+    if (lda < 0 || ldg < 0 || (reinterpret_cast<uintptr_t>(workspace) & 15)) return TRT_E_LAYOUT;
+    if (!stride_fits(lda, size) || !stride_fits(ldg, size) || !stride_fits(N, size) || !stride_fits(K, size) || T >= (int64_t)1 << 31 ||
+        E >= (int64_t)1 << 31)
+        return TRT_E_RANGE;
+    g = {};
+    g.x = a, g.y = g_, g.out = d;
+    g.sizes = {sizes, wide_sizes, E, T};
+    g.M = K, g.N = N, g.ldx = lda, g.ldy = ldg;
+    return TRT_OK;
+}
+
+int rows_product(const void *a, const void *b, const void *sizes, void *c, int64_t T, int64_t E, int64_t K, int64_t N, int64_t lda,
+                 const int64_t sb[3], int dtype, int wide_sizes, int tile, const Workspace &w, void *stream) {
+    GmmArgs g;
+    bool inner;
+    const int status = rows_args(a, b, sizes, c, T, E, K, N, lda, sb, dtype, wide_sizes, tile, w.p, w.query != nullptr, g, inner);
+    return status ? status : dispatch(g, E, T, false, inner, dtype, tile, w, stream);
 }
 
 int weights_product(const void *a, const void *g_, const void *sizes, void *d, int64_t T, int64_t E, int64_t K, int64_t N, int64_t lda,
                     int64_t ldg, int dtype, int wide_sizes, int tile, const Workspace &w, void *stream) {
-    const size_t size = type_size(dtype);
-    if (!a || !g_ || T <= 0 || E <= 0 || K <= 0 || N <= 0 || !size || tile < 0 || tile > TRT_GMM_TILES) return TRT_E_INVALID;
-    if (!w.query && (!sizes || !d)) return TRT_E_INVALID;
-    if (lda < 0 || ldg < 0 || (reinterpret_cast<uintptr_t>(w.p) & 15)) return TRT_E_LAYOUT;
-    if (!stride_fits(lda, size) || !stride_fits(ldg, size) || !stride_fits(N, size) || !stride_fits(K, size) || T >= (int64_t)1 << 31 ||
-        E >= (int64_t)1 << 31)
-        return TRT_E_RANGE;
-    GmmArgs g = {};
-    g.x = a, g.y = g_, g.out = d;
-    g.sizes = {sizes, wide_sizes, E, T};
-    g.M = K, g.N = N, g.ldx = lda, g.ldy = ldg;
-    return dispatch(g, E, T, true, false, dtype, tile, w, stream);
+    GmmArgs g;
+    const int status = weights_args(a, g_, sizes, d, T, E, K, N, lda, ldg, dtype, wide_sizes, tile, w.p, w.query != nullptr, g);
+    return status ? status : dispatch(g, E, T, true, false, dtype, tile, w, stream);
+}
+
+// The rows' product with b's last two axes exchanged and the weights' product; the arguments of both are looked at before anything is
+// enqueued.
+int both_products(const void *g, const void *a, const void *b, const void *sizes, void *da, void *db, int64_t T, int64_t E, int64_t K,
+                  int64_t N, int64_t ldg, int64_t lda, const int64_t sb[3], int dtype, int wide_sizes, const Workspace &ws, void *stream) {
+    if (!sb) return TRT_E_INVALID;
+    const int64_t st[3] = {sb[0], sb[2], sb[1]};
+    GmmArgs r, w;
+    bool inner;
+    const bool query = ws.query != nullptr;
+    int status = weights_args(a, g, sizes, db, T, E, K, N, lda, ldg, dtype, wide_sizes, 0, ws.p, query, w);
+    if (!status) status = rows_args(g, b, sizes, da, T, E, N, K, ldg, st, dtype, wide_sizes, 0, ws.p, query, r, inner);
+    if (status) return status;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (dtype) {
+        case TRT_BF16: return gmm_grad_bf16(r, w, E, T, inner, ws, s);
+        case TRT_F16: return gmm_grad_f16(r, w, E, T, inner, ws, s);
+        default: return gmm_grad_f32(r, w, E, T, inner, ws, s);
+    }
 }
 
 }  // namespace
@@ -82,25 +118,15 @@ extern "C" size_t trt_gmm_weights_workspace_bytes(const void *a, const void *g, 
     return bytes;
 }
 
-// Both gradients in one call: the rows' product with b's last two axes exchanged, then the weights' product, which may use the same
-// workspace after it.
 extern "C" int trt_gmm_grad(const void *g, const void *a, const void *b, const void *sizes, void *da, void *db, int64_t T, int64_t E,
                             int64_t K, int64_t N, int64_t ldg, int64_t lda, const int64_t sb[3], int dtype, int wide_sizes, void *workspace,
                             size_t workspace_bytes, void *stream) {
-    if (!sb || !db) return TRT_E_INVALID;
-    const int64_t st[3] = {sb[0], sb[2], sb[1]};
-    size_t none = 0;  // the second product's arguments are looked at before the first is enqueued
-    int status = weights_product(a, g, sizes, db, T, E, K, N, lda, ldg, dtype, wide_sizes, 0, {workspace, workspace_bytes, &none}, stream);
-    if (!status) status = rows_product(g, b, sizes, da, T, E, N, K, ldg, st, dtype, wide_sizes, 0, {workspace, workspace_bytes, nullptr}, stream);
-    if (!status) status = weights_product(a, g, sizes, db, T, E, K, N, lda, ldg, dtype, wide_sizes, 0, {workspace, workspace_bytes, nullptr}, stream);
-    return status;
+    return both_products(g, a, b, sizes, da, db, T, E, K, N, ldg, lda, sb, dtype, wide_sizes, {workspace, workspace_bytes, nullptr}, stream);
 }
 
 extern "C" size_t trt_gmm_grad_workspace_bytes(const void *g, const void *a, const void *b, int64_t T, int64_t E, int64_t K, int64_t N,
                                                int64_t ldg, int64_t lda, const int64_t sb[3], int dtype) {
-    if (!sb) return 0;
-    const int64_t st[3] = {sb[0], sb[2], sb[1]};
-    const size_t rows = trt_gmm_workspace_bytes(g, b, T, E, N, K, ldg, st, dtype, 0);
-    const size_t weights = trt_gmm_weights_workspace_bytes(a, g, T, E, K, N, lda, ldg, dtype, 0);
-    return rows > weights ? rows : weights;
+    size_t bytes = 0;
+    both_products(g, a, b, nullptr, nullptr, nullptr, T, E, K, N, ldg, lda, sb, dtype, 0, {nullptr, 0, &bytes}, nullptr);
+    return bytes;
 }

@@ -7,4 +7,8 @@ int gmm_bf16(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_i
     return launch_gmm_type<__bf16>(g, E, T_rows, weights, y_inner, tile, w, s);
 }
 
+int gmm_grad_bf16(const GmmArgs &r, const GmmArgs &w, int64_t E, int64_t T_rows, bool y_inner, const Workspace &ws, hipStream_t s) {
+    return launch_gmm_grad_type<__bf16>(r, w, E, T_rows, y_inner, ws, s);
+}
+
 }  // namespace trt

@@ -142,15 +142,14 @@ struct PadJob {
     uint32_t total;        // chunks in all
 };
 template <typename T>
-__global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b, uint32_t a_blocks) {
-    const bool second = blockIdx.x >= a_blocks;
-    const PadJob &j = second ? b : a;
-    const uint32_t i = (blockIdx.x - (second ? a_blocks : 0)) * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b, PadJob c, uint32_t a_blocks, uint32_t ab_blocks) {
+    const PadJob &j = blockIdx.x < a_blocks ? a : blockIdx.x < ab_blocks ? b : c;
+    const uint32_t i = (blockIdx.x - (blockIdx.x < a_blocks ? 0 : blockIdx.x < ab_blocks ? a_blocks : ab_blocks)) * 256 + threadIdx.x;
     if (i >= j.total) return;
     constexpr int V = 16 / sizeof(T);
-    const uint32_t row = divide(i, j.chunks), c = (i - row * j.chunks.d) * V, e = divide(row, j.rows);
-    const T *p = static_cast<const T *>(j.from) + e * j.group + (row - e * j.rows.d) * j.ld + c;
-    static_cast<uintx4 *>(j.to)[i] = load_chunk(p, j.n - c);
+    const uint32_t row = divide(i, j.chunks), at = (i - row * j.chunks.d) * V, e = divide(row, j.rows);
+    const T *p = static_cast<const T *>(j.from) + e * j.group + (row - e * j.rows.d) * j.ld + at;
+    static_cast<uintx4 *>(j.to)[i] = load_chunk(p, j.n - at);
 }
 
 struct PadPlan {
@@ -171,29 +170,34 @@ PadPlan plan_pads(const GmmArgs &g, int64_t E, int64_t T_rows, double us, double
     return p;
 }
 
-template <typename T, int XL, int YL>
-int apply_pads(GmmArgs &g, int64_t E, int64_t T_rows, const PadPlan &p, void *workspace, hipStream_t s) {
-    if (!p.bytes) return 0;
+// A copy of `groups` matrices to `to`, which moves on behind it; from, ld and group become the copy's.
+template <typename T>
+PadJob pad_job(bool wanted, const void *&from, int64_t &ld, int64_t *group, int64_t n, int64_t rows, int64_t groups, char *&to) {
+    PadJob j = {};
+    if (!wanted) return j;
     constexpr int64_t V = 16 / sizeof(T);
-    char *to = static_cast<char *>(workspace);
-    auto job = [&](bool wanted, const void *&from, int64_t &ld, int64_t &group, int64_t n, int64_t rows, int64_t groups) {
-        PadJob j = {};
-        if (!wanted) return j;
-        const int64_t chunks = ceil_div(n, V);
-        j = {from, to, n, ld, group, divider((uint32_t)chunks), divider((uint32_t)rows), (uint32_t)(groups * rows * chunks)};
-        from = to;
-        to += (size_t)j.total * 16;
-        ld = chunks * V;
-        group = rows * ld;
-        return j;
-    };
-    int64_t none = 0;
-    const bool matrices = XL == kInner;
-    const PadJob a = job(p.x, g.x, g.ldx, none, XL == kInner ? g.K : g.M, T_rows, 1);
-    const PadJob b = job(p.y, g.y, g.ldy, matrices ? g.y_group : none, YL == kInner ? g.K : g.N, !matrices ? T_rows : YL == kInner ? g.N : g.K,
-                         matrices ? E : 1);
-    const uint32_t a_blocks = (uint32_t)ceil_div(a.total, 256), b_blocks = (uint32_t)ceil_div(b.total, 256);
-    hipLaunchKernelGGL(pad_rows_kernel<T>, dim3(a_blocks + b_blocks), dim3(256), 0, s, a, b, a_blocks);
+    const int64_t chunks = ceil_div(n, V);
+    j = {from, to, n, ld, group ? *group : 0, divider((uint32_t)chunks), divider((uint32_t)rows), (uint32_t)(groups * rows * chunks)};
+    from = to;
+    to += (size_t)j.total * 16;
+    ld = chunks * V;
+    if (group) *group = rows * ld;
+    return j;
+}
+// The rows' operand or, of a rows' product, the matrices.
+template <typename T, int XL>
+PadJob pad_x(bool wanted, GmmArgs &g, int64_t T_rows, char *&to) {
+    return pad_job<T>(wanted, g.x, g.ldx, nullptr, XL == kInner ? g.K : g.M, T_rows, 1, to);
+}
+template <typename T, int XL, int YL>
+PadJob pad_y(bool wanted, GmmArgs &g, int64_t E, int64_t T_rows, char *&to) {
+    if (XL == kOuter) return pad_job<T>(wanted, g.y, g.ldy, nullptr, g.N, T_rows, 1, to);
+    return pad_job<T>(wanted, g.y, g.ldy, &g.y_group, YL == kInner ? g.K : g.N, YL == kInner ? g.N : g.K, E, to);
+}
+template <typename T>
+int launch_pads(const PadJob &a, const PadJob &b, const PadJob &c, hipStream_t s) {
+    const uint32_t a_blocks = (uint32_t)ceil_div(a.total, 256), ab = a_blocks + (uint32_t)ceil_div(b.total, 256), all = ab + (uint32_t)ceil_div(c.total, 256);
+    hipLaunchKernelGGL(pad_rows_kernel<T>, dim3(all), dim3(256), 0, s, a, b, c, a_blocks, ab);
     return (int)hipGetLastError();
 }
 
@@ -203,37 +207,45 @@ struct Workspace {
     size_t *query;  // not null: only say how many are wanted
 };
 
+// How a product is made: its tile, the rows of a piece (0: groups are whole), the copies, and the bytes of the pieces' sums.
+struct GmmPlan {
+    int tile;
+    int64_t piece;
+    PadPlan pads;
+    size_t partial;
+};
+
 // x: the rows' operand (a; a transposed for the weights), y: the matrices or g.
 template <typename T, int XL, int YL>
-int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &w, hipStream_t s) {
+GmmPlan plan_gmm(const GmmArgs &g, int64_t E, int64_t T_rows, int tile) {
+    GmmPlan p = {tile, 0, {false, false, 0}, 0};
     double us = 0.0;
-    int64_t piece = 0;
     if constexpr (XL == kOuter) {
         if (tile == 0) {
-            tile = choose_weights_tile<T>(E, g.M, g.N);
-            piece = choose_weights_piece<T>(T_rows, E, g.M, g.N, tile);
+            p.tile = choose_weights_tile<T>(E, g.M, g.N);
+            p.piece = choose_weights_piece<T>(T_rows, E, g.M, g.N, p.tile);
         }
         us = 10.0 + 2.0 * (double)T_rows * (double)g.M * (double)g.N / (sizeof(T) == 4 ? 60e6 : 900e6);
     } else {
         const int best = choose_gmm_tile<T>(T_rows, E, g.N, g.K, YL == kInner, &us);
-        if (tile == 0) tile = best;
+        if (tile == 0) p.tile = best;
     }
     // few rows are bound by reading the matrices, and a copy reads and writes them
-    const bool few = XL == kInner && tile >= 2 && tile <= 4;
-    const PadPlan pads = few ? PadPlan{false, false, 0} : plan_pads<T, XL, YL>(g, E, T_rows, us, XL == kOuter ? 1.2 : YL == kOuter ? 0.8 : 0.5);
-    const size_t partial = piece ? (size_t)(most_pieces(T_rows, E, piece) * ceil_div(g.M, 128) * ceil_div(g.N, 128)) * (128 * 128 * sizeof(float)) : 0;
-    if (w.query) {
-        *w.query = pads.bytes + partial;
-        return TRT_OK;
-    }
-    const bool work = w.p && w.bytes >= pads.bytes + partial;  // without a workspace operands are read as they are, and rows not cut
-    if (work && partial) g.partial = reinterpret_cast<float *>(static_cast<char *>(w.p) + pads.bytes), g.piece = divider((uint32_t)piece), tile = 1;
-    bool aligned = chunks_aligned<T>(g.x, {g.ldx, XL == kInner ? g.K : g.M}) && chunks_aligned<T>(g.y, {g.ldy, g.y_group, YL == kInner ? g.K : g.N});
-    if (pads.bytes && work) {
-        const int status = apply_pads<T, XL, YL>(g, E, T_rows, pads, w.p, s);
-        if (status) return status;
-        aligned = true;
-    }
+    const bool few = XL == kInner && p.tile >= 2 && p.tile <= 4;
+    if (!few) p.pads = plan_pads<T, XL, YL>(g, E, T_rows, us, XL == kOuter ? 1.2 : YL == kOuter ? 0.8 : 0.5);
+    if (p.piece) p.partial = (size_t)(most_pieces(T_rows, E, p.piece) * ceil_div(g.M, 128) * ceil_div(g.N, 128)) * (128 * 128 * sizeof(float));
+    return p;
+}
+
+template <typename T, int XL>
+bool x_aligned(const GmmArgs &g) { return chunks_aligned<T>(g.x, {g.ldx, XL == kInner ? g.K : g.M}); }
+template <typename T, int YL>
+bool y_aligned(const GmmArgs &g) { return chunks_aligned<T>(g.y, {g.ldy, g.y_group, YL == kInner ? g.K : g.N}); }
+
+// aligned: both operands' rows are whole chunks on their boundaries.
+template <typename T, int XL, int YL>
+int run_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, bool aligned, hipStream_t s) {
+    if (g.partial) tile = 1;
     if constexpr (XL == kInner) {
         switch (tile) {
             case 2: return aligned ? launch_gmm_few_rows<T, YL>(g, E, T_rows, s) : launch_gmm_few<T, YL, 1, false>(g, E, T_rows, s);
@@ -267,6 +279,60 @@ int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &
     return status;
 }
 
+template <typename T, int XL, int YL>
+int launch_gmm(GmmArgs g, int64_t E, int64_t T_rows, int tile, const Workspace &w, hipStream_t s) {
+    const GmmPlan p = plan_gmm<T, XL, YL>(g, E, T_rows, tile);
+    if (w.query) {
+        *w.query = p.pads.bytes + p.partial;
+        return TRT_OK;
+    }
+    bool aligned = x_aligned<T, XL>(g) && y_aligned<T, YL>(g);
+    if (w.p && w.bytes >= p.pads.bytes + p.partial) {  // without a workspace operands are read as they are, and groups not cut
+        char *to = static_cast<char *>(w.p);
+        if (p.pads.bytes) {
+            const PadJob x = pad_x<T, XL>(p.pads.x, g, T_rows, to), y = pad_y<T, XL, YL>(p.pads.y, g, E, T_rows, to);
+            const int status = launch_pads<T>(x, y, {}, s);
+            if (status) return status;
+            aligned = true;
+        }
+        if (p.partial) g.partial = reinterpret_cast<float *>(to), g.piece = divider((uint32_t)p.piece);
+    }
+    return run_gmm<T, XL, YL>(g, E, T_rows, p.tile, aligned, s);
+}
+
+// Both gradients: r is a's (its x is g), w the matrices' (its y is g).  g is copied once for both, and all copies are one launch.
+template <typename T, int YL>
+int launch_gmm_grad(GmmArgs r, GmmArgs w, int64_t E, int64_t T_rows, const Workspace &ws, hipStream_t s) {
+    const GmmPlan pr = plan_gmm<T, kInner, YL>(r, E, T_rows, 0), pw = plan_gmm<T, kOuter, kOuter>(w, E, T_rows, 0);
+    const bool pad_g = pr.pads.x || pw.pads.y;
+    bool g_ok = x_aligned<T, kInner>(r), b_ok = y_aligned<T, YL>(r), a_ok = x_aligned<T, kOuter>(w);
+    GmmArgs rp = r, wp = w;
+    char *const base = static_cast<char *>(ws.p), *to = base;
+    const PadJob g = pad_x<T, kInner>(pad_g, rp, T_rows, to), b = pad_y<T, kInner, YL>(pr.pads.y, rp, E, T_rows, to), a = pad_x<T, kOuter>(pw.pads.x, wp, T_rows, to);
+    const size_t copies = (size_t)g.total * 16 + (size_t)b.total * 16 + (size_t)a.total * 16;
+    if (ws.query) {
+        *ws.query = copies + pw.partial;
+        return TRT_OK;
+    }
+    if (ws.p && ws.bytes >= copies + pw.partial) {
+        if (pad_g) wp.y = rp.x, wp.ldy = rp.ldx;
+        r = rp, w = wp;
+        if (copies) {
+            const int status = launch_pads<T>(g, b, a, s);
+            if (status) return status;
+            g_ok = g_ok || pad_g, b_ok = b_ok || pr.pads.y, a_ok = a_ok || pw.pads.x;
+        }
+        if (pw.partial) w.partial = reinterpret_cast<float *>(base + copies), w.piece = divider((uint32_t)pw.piece);
+    }
+    const int status = run_gmm<T, kInner, YL>(r, E, T_rows, pr.tile, g_ok && b_ok, s);
+    return status ? status : run_gmm<T, kOuter, kOuter>(w, E, T_rows, pw.tile, a_ok && g_ok, s);
+}
+
+template <typename T>
+int launch_gmm_grad_type(const GmmArgs &r, const GmmArgs &w, int64_t E, int64_t T_rows, bool y_inner, const Workspace &ws, hipStream_t s) {
+    return y_inner ? launch_gmm_grad<T, kInner>(r, w, E, T_rows, ws, s) : launch_gmm_grad<T, kOuter>(r, w, E, T_rows, ws, s);
+}
+
 template <typename T>
 int launch_gmm_type(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s) {
     if (weights) return launch_gmm<T, kOuter, kOuter>(g, E, T_rows, tile, w, s);
@@ -276,5 +342,9 @@ int launch_gmm_type(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, b
 int gmm_bf16(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s);
 int gmm_f16(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s);
 int gmm_f32(const GmmArgs &g, int64_t E, int64_t T_rows, bool weights, bool y_inner, int tile, const Workspace &w, hipStream_t s);
+
+int gmm_grad_bf16(const GmmArgs &r, const GmmArgs &w, int64_t E, int64_t T_rows, bool y_inner, const Workspace &ws, hipStream_t s);
+int gmm_grad_f16(const GmmArgs &r, const GmmArgs &w, int64_t E, int64_t T_rows, bool y_inner, const Workspace &ws, hipStream_t s);
+int gmm_grad_f32(const GmmArgs &r, const GmmArgs &w, int64_t E, int64_t T_rows, bool y_inner, const Workspace &ws, hipStream_t s);
 
 }  // namespace trt
