@@ -317,8 +317,9 @@ int trt_mm_bf16(const float *a, const float *b, float *c, int64_t m, int64_t k, 
  * Operands whose base, strides and rows are multiples of 16 bytes are fastest.  Others are read as they lie, or, where that pays,
  * copied first: that takes a workspace of trt_gmm_workspace_bytes(...) or trt_gmm_weights_workspace_bytes(...) bytes for the
  * same arguments (usually 0), 16-byte aligned; without it they are read as they lie.  trt_gmm_weights also cuts long groups into
- * pieces there where tiles are few, whose sums it adds in a fixed order; without a workspace it does not.  A row may be at most 8 MiB long
- * or apart, T and E below 2^31 (TRT_E_RANGE).  tile: 0 = choose by shape, 1..TRT_GMM_TILES force a tile (experiments, tests).
+ * pieces there where tiles are few, whose sums it adds in a fixed order (they take at most 256 MiB, or half of what operands
+ * and result take); without a workspace it does not.  A row may be at most 8 MiB long or apart, T and E below 2^31
+ * (TRT_E_RANGE).  tile: 0 = choose by shape, 1..TRT_GMM_TILES force a tile (experiments, tests).
  */
 #define TRT_GMM_TILES 5
 int trt_gmm(const void *a, const void *b, const void *sizes, void *c, int64_t T, int64_t E, int64_t K,

@@ -1,0 +1,66 @@
+"""Workspaces of the grouped products' gradients, without a GPU: the queries are host only."""
+
+import ctypes
+import math
+import random
+
+import pytest
+
+from triturus_amd import _lib
+
+F32, F16, BF16 = _lib.TRT_F32, _lib.TRT_F16, _lib.TRT_BF16
+SIZE = {F32: 4, F16: 2, BF16: 2}
+AT = 1 << 20  # an address on the boundaries; never dereferenced
+
+
+def copies(T, K, N, dtype):
+    """Bytes of both operands in rows of whole 16-byte chunks."""
+    values = 16 // SIZE[dtype]
+    return 16 * T * (-(-K // values) + -(-N // values))
+
+
+def weights(T, E, K, N, dtype, a=AT):
+    return _lib.load().trt_gmm_weights_workspace_bytes(a, AT, T, E, K, N, K, N, dtype, 0)
+
+
+def grad(T, E, K, N, dtype):
+    sb = (ctypes.c_int64 * 3)(K * N, N, 1)
+    return _lib.load().trt_gmm_grad_workspace_bytes(AT, AT, AT, T, E, K, N, N, K, sb, dtype)
+
+
+def held(T, E, K, N, dtype):
+    return (T * (K + N) + E * K * N) * SIZE[dtype]
+
+
+def shapes(count, seed):
+    rng = random.Random(seed)
+
+    def between(lo, hi):
+        return int(math.exp(rng.uniform(math.log(lo), math.log(hi))))
+
+    for _ in range(count):
+        E = between(1, 600)
+        yield between(1, 1 << 22), E, between(1, 9000), between(1, 9000), rng.choice([F32, F16, BF16])
+
+
+@pytest.mark.parametrize("T,E,K,N,dtype", [(16384, 8, 4097, 4096, F32), (104869, 8, 7911, 8161, F32), (16384, 8, 4104, 4096, F32), (16384, 8, 2056, 2048, F32),
+                                           (16384, 8, 4097, 4095, BF16), (26870, 18, 849, 2096, BF16), (6067, 9, 616, 3000, BF16)])
+def test_many_tiles_are_not_cut(T, E, K, N, dtype):
+    """Where the tiles take several rounds of all CUs, long and short groups average out and a cut gains nothing."""
+    aligned = K % 8 == 0 and N % 8 == 0
+    assert weights(T, E, K, N, dtype) <= (0 if aligned else copies(T, K, N, dtype))
+
+
+def test_pieces_take_a_bounded_workspace():
+    """The sums of pieces: at most 256 MiB, or half of what the call's operands and result take."""
+    for T, E, K, N, dtype in shapes(20000, 5):
+        most = max(256 << 20, held(T, E, K, N, dtype) // 2)
+        assert weights(T, E, K, N, dtype) <= most + copies(T, K, N, dtype), (T, E, K, N, dtype)
+        b = 16 * max(E * K * -(-N * SIZE[dtype] // 16), E * N * -(-K * SIZE[dtype] // 16))  # b may be copied too
+        assert grad(T, E, K, N, dtype) <= most + copies(T, K, N, dtype) + b, (T, E, K, N, dtype)
+
+
+def test_few_tiles_under_many_rows_are_still_cut():
+    for T, E, K, N, dtype in ((16384, 1, 512, 512, BF16), (16384, 1, 512, 512, F32), (32768, 1, 2048, 1024, BF16), (1500000, 200, 80, 632, BF16),
+                              (500000, 460, 16, 336, BF16), (350000, 500, 240, 128, F32)):
+        assert weights(T, E, K, N, dtype) > 0

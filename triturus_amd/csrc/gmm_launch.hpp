@@ -100,27 +100,33 @@ int choose_weights_tile(int64_t E, int64_t K, int64_t N) {
 // choice above.  The pieces' sums are added in order by another launch.  Estimates in microseconds, fitted to pieces of a
 // 1/32 .. 1 of the mean group on 90 random shapes: a step of 64 bytes a row with up to one, two or more workgroups on a CU, both
 // launches, a piece's tile written and read, and without pieces how much longer the longest of several groups is than their mean.
-// The choice is 6 to 7 % behind the best pieces on average, none 2.3 times (16384 rows, 512 x 512 of bf16: 175 us, 29 in pieces;
-// 16 uneven groups, 256 x 512: 48 and 26).
+// That is charged for up to one step of a full CU, two where more than 64 groups are taken as they come: beyond it the tiles come in
+// rounds, over which long and short groups average out (8 groups of 2048 rows, 2056 x 2048 of fp32: 1077 us whole, 1213 in pieces;
+// 9 of 674, 616 x 3000 of bf16: 36 and 72).  The pieces' sums may take 256 MiB, or half of what operands and result take.
+// On 920 random shapes, up to 6000 tiles and 4 million rows, the choice is 6 % behind the best pieces on average and 2.9 times on the
+// worst, whole groups 1.6 and 31 times (16384 rows, 512 x 512 of bf16: 175 us, 29 in pieces; 16 uneven groups, 256 x 512: 48 and 26).
+constexpr double kMostSums = 256 << 20;
 template <typename T>
 int64_t choose_weights_piece(int64_t T_rows, int64_t E, int64_t K, int64_t N, int tile) {
     constexpr bool F32 = sizeof(T) == 4;
     if (tile == 5) return 0;
     const double matrix = (double)(ceil_div(K, 128) * ceil_div(N, 128)), mid = (double)E * matrix;
-    const double small = ceil((double)(E * ceil_div(K, 64) * ceil_div(N, 64)) / 256), longest = 1.0 + (F32 ? 0.26 : 0.50) * log2((double)(E < 16 ? E : 16));
-    auto step = [](double workgroups) {
-        const double one = F32 ? 1.05 : 0.36, two = F32 ? 1.93 : 0.57, three = F32 ? 2.79 : 0.855;
-        return workgroups <= 256 ? one : workgroups <= 512 ? two : three * ceil(workgroups / 256) / 3;
-    };
+    const double small = ceil((double)E * (double)(ceil_div(K, 64) * ceil_div(N, 64)) / 256), longest = 1.0 + (F32 ? 0.26 : 0.50) * log2((double)(E < 16 ? E : 16));
+    constexpr double one = F32 ? 1.05 : 0.36, two = F32 ? 1.93 : 0.57, three = F32 ? 2.79 : 0.855;
+    auto step = [](double workgroups) { return workgroups <= 256 ? one : workgroups <= 512 ? two : three * ceil(workgroups / 256) / 3; };
+    auto larger = [](double a, double b) { return a > b ? a : b; };
     const double steps = (double)ceil_div(ceil_div(T_rows, E) * (int64_t)sizeof(T), 64);
-    const double least = F32 ? 0.382 : 0.314, shared = (F32 ? 0.22 : 0.122) * small;
-    double best = 0.97 * (3.3 + longest * steps * (tile == 2 ? (least > shared ? least : shared) : step(mid)));
+    const double mean = tile == 2 ? larger(F32 ? 0.382 : 0.314, (F32 ? 0.22 : 0.122) * small) : step(mid);
+    const double held = ((double)T_rows * (double)(K + N) + (double)E * (double)K * (double)N) * (double)sizeof(T);
+    const double full = E <= kWave ? three : 2 * three;
+    double best = 0.97 * (3.3 + steps * larger(mean, longest * (mean < full ? mean : full)));
     int64_t rows = 0;
     for (int64_t p = 1; p <= 32; ++p) {
         const int64_t len = ceil_div(ceil_div(T_rows, E * p), 32) * 32;
         if (len * (int64_t)sizeof(T) < 4 * 64) break;
+        if ((double)most_pieces(T_rows, E, len) * matrix * (128 * 128 * sizeof(float)) > larger(kMostSums, 0.5 * held)) break;
         const double n = E == 1 ? (double)ceil_div(T_rows, len) : (double)(T_rows / len) + 0.5 * (double)E, w = n * matrix;
-        const double us = (F32 ? 13.3 : 11.5) + (double)(len * (int64_t)sizeof(T) / 64) * step(w) + w * 0.021;
+        const double us = (F32 ? 13.3 : 11.5) + (double)(len * (int64_t)sizeof(T) / 64) * step(w) + w * 0.024;
         if (us < best) best = us, rows = len;
     }
     return rows;
