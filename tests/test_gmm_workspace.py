@@ -64,3 +64,41 @@ def test_few_tiles_under_many_rows_are_still_cut():
     for T, E, K, N, dtype in ((16384, 1, 512, 512, BF16), (16384, 1, 512, 512, F32), (32768, 1, 2048, 1024, BF16), (1500000, 200, 80, 632, BF16),
                               (500000, 460, 16, 336, BF16), (350000, 500, 240, 128, F32)):
         assert weights(T, E, K, N, dtype) > 0
+
+
+def test_the_library_alone_decides_on_pieces():
+    """gmm.py asks for no workspace only where the library would want none: groups of 32 rows or fewer on average, operands on the boundaries."""
+    from triturus_amd.gmm import _few_rows
+
+    rng = random.Random(9)
+    wanted = 0
+    for T, E, K, N, dtype in shapes(40000, 8):
+        K, N = -(-K // 8) * 8, -(-N // 8) * 8
+        if rng.random() < 0.3:  # next to the border
+            T = max(1, min((1 << 31) - 1, 32 * E + rng.randint(-3, 40 * E)))
+        if weights(T, E, K, N, dtype):
+            wanted += 1
+            assert not _few_rows(T, E), (T, E, K, N, dtype)
+    assert wanted > 5000 and _few_rows(64, 2) and not _few_rows(65, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,K,N,dtype", [(3784, 3, 1640, 1760, BF16), (7302, 16, 720, 888, F32)])
+def test_the_cut_does_not_depend_on_alignment(dev, T, E, K, N, dtype):
+    """The same operands on and off the 16-byte boundaries: the same pieces, so the same sums bit for bit."""
+    import torch
+
+    from triturus_amd.gmm import gmm_grad
+
+    dtype = {code: t for t, code in _lib.DTYPE_CODES.items()}[dtype]
+    a, g, b = (torch.randn(*shape, device=dev).to(dtype) for shape in ((T, K), (T, N), (E, K, N)))
+    sizes = torch.full((E,), T // E, dtype=torch.int32, device=dev)
+    off = torch.empty(T * K + 1, device=dev, dtype=dtype)[1:].view(T, K).copy_(a)
+    assert a.data_ptr() % 16 == 0 and off.data_ptr() % 16 != 0
+    want = torch.stack([a[e * (T // E):(e + 1) * (T // E)].double().T @ g[e * (T // E):(e + 1) * (T // E)].double() for e in range(E)])
+    d = gmm_grad(g, a, b, sizes)[1]
+    assert torch.equal(gmm_grad(g, off, b, sizes)[1], d)
+    # fp32 sums of T / E products, each addition within 2^-23 of the running magnitudes, and the result's own rounding
+    size = torch.stack([a[e * (T // E):(e + 1) * (T // E)].double().abs().T @ g[e * (T // E):(e + 1) * (T // E)].double().abs() for e in range(E)])
+    bound = (T // E + 1) * 2.0 ** -23 * size + torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2 ** -8)
+    assert ((d.double() - want).abs() <= bound).all()

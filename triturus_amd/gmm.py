@@ -69,9 +69,10 @@ def _matrices(b: torch.Tensor) -> torch.Tensor:
     return dense(b)
 
 
-def _few_tiles(T: int, E: int, K: int, N: int) -> bool:
-    """Whether the library may cut the rows of the matrices' gradient, which takes a workspace."""
-    return E * K * N <= 1 << 23 and T >= 128 * E
+def _few_rows(T: int, E: int) -> bool:
+    """Whether the library cuts no group into pieces, whatever the matrices: a piece has at least 256 bytes of a column (64 rows of
+    fp32, 128 of 16-bit types) and is a multiple of 32 rows, and groups of at most 32 rows on average leave pieces of 32."""
+    return T <= 32 * E
 
 
 def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:
@@ -128,7 +129,7 @@ def _weights(a: torch.Tensor, g: torch.Tensor, sizes: torch.Tensor, tile: int = 
     lib, code = _lib.load(), _lib.DTYPE_CODES[dtype]
     pa, pg, lda, ldg = a.data_ptr(), g.data_ptr(), a.stride(0), g.stride(0)
     ws_ptr, nbytes, ws = None, 0, None
-    if (pa | pg) & 15 or (K | N | lda | ldg) & 7 or _few_tiles(T, E, K, N):  # a copy or a cut may pay
+    if (pa | pg) & 15 or (K | N | lda | ldg) & 7 or not _few_rows(T, E):  # a copy or a cut may pay
         nbytes = lib.trt_gmm_weights_workspace_bytes(pa, pg, T, E, K, N, lda, ldg, code, tile)
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -183,7 +184,7 @@ def gmm_grad(g: torch.Tensor, a: torch.Tensor, b: torch.Tensor, sizes: torch.Ten
     lib, code = _lib.load(), _lib.DTYPE_CODES[a.dtype]
     pg, pa, pb, ldg, lda, sb = g.data_ptr(), a.data_ptr(), b.data_ptr(), g.stride(0), a.stride(0), _lib.strides3(b)
     ws_ptr, nbytes, ws = None, 0, None
-    if (pg | pa | pb) & 15 or (K | N | ldg | lda | sb[0] | (sb[2] if sb[1] == 1 else sb[1])) & 7 or _few_tiles(T, E, K, N):  # a copy or a cut may pay
+    if (pg | pa | pb) & 15 or (K | N | ldg | lda | sb[0] | (sb[2] if sb[1] == 1 else sb[1])) & 7 or not _few_rows(T, E):  # a copy or a cut may pay
         nbytes = lib.trt_gmm_grad_workspace_bytes(pg, pa, pb, T, E, K, N, ldg, lda, sb, code)
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
