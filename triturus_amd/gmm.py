@@ -153,6 +153,8 @@ class _Gmm(torch.autograd.Function):
     def backward(ctx, g):
         refuse_capture("gmm")
         a, b, sizes = ctx.saved_tensors
+        if ctx.needs_input_grad[0] and ctx.needs_input_grad[1]:
+            return *gmm_grad(g, a, b, sizes), None
         da = _forward(g, b.transpose(1, 2), sizes) if ctx.needs_input_grad[0] else None
         db = _weights(a, g, sizes) if ctx.needs_input_grad[1] else None
         return da, db, None
