@@ -66,3 +66,20 @@ def test_backward_is_gmm_grad(dev, K, N, dtype, layout):
     module.gmm(a, b, sizes).backward(g)
     da, db = module.gmm_grad(g, a.detach(), b.detach(), sizes)
     assert torch.equal(a.grad, da) and torch.equal(b.grad, db)
+
+
+@pytest.mark.parametrize("a_grad", [True, False])
+def test_one_gradient_keeps_one_operand(calls, a_grad):
+    """The other operand is neither kept alive nor guarded against changes in place."""
+    a, b, s = operands(a_grad, not a_grad)
+    c = module._Gmm.apply(a, b, s)
+    kept = c.grad_fn.saved_tensors
+    assert kept[0] is None if a_grad else kept[1] is None
+    g = torch.randn_like(c)
+    want = rows_product(g, b.transpose(1, 2), s) if a_grad else weights_product(a, g, s)
+    del calls[:]
+    with torch.no_grad():
+        (a if a_grad else b).mul_(2)  # the operand whose own values its gradient does not need
+    c.backward(g)
+    assert torch.equal(a.grad if a_grad else b.grad, want)
+    assert calls == ["_forward" if a_grad else "_weights"]

@@ -145,7 +145,8 @@ def _weights(a: torch.Tensor, g: torch.Tensor, sizes: torch.Tensor, tile: int = 
 class _Gmm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, sizes):
-        ctx.save_for_backward(a, b, sizes)
+        need = ctx.needs_input_grad  # a gradient takes the other operand's values alone
+        ctx.save_for_backward(a if need[1] else None, b if need[0] else None, sizes)
         return _forward(a, b, sizes)
 
     @staticmethod
