@@ -14,12 +14,14 @@ Groups may be empty.  Sizes that are negative or reach past T in sum are clamped
 
 ``gmm`` takes part in autograd.  Under HIP graph capture it refuses operands that require a gradient: capture
 ``gmm`` on detached operands and ``gmm_grad`` instead (a backward pass of autograd captured while another graph
-of the same leaves is alive ends the process inside torch).
+of the same leaves is alive ends the process inside torch).  ``gmm_grad`` itself takes no part in autograd.  Forward-mode
+derivatives are refused.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from triturus_amd import _lib
@@ -38,6 +40,14 @@ def refuse_capture(op: str) -> None:
             f"{op}: operands that require a gradient are refused under graph capture; "
             f"capture {op} on detached operands and {op}_grad"
         )
+
+
+def refuse_tangents(op: str, *tensors: torch.Tensor) -> None:
+    """Operands with a forward-mode tangent: they do not require a gradient, and the result would lose it without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside of dual levels no tensor has one
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{op} has no forward-mode derivative: pass the primal of its operands")
 
 
 # The kernels address 256 rows of a tile with 31-bit byte offsets: rows further apart than this many bytes are copied
@@ -75,7 +85,7 @@ def _few_rows(T: int, E: int) -> bool:
     return T <= 32 * E
 
 
-def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:
+def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor, op: str = "gmm") -> None:
     sa, sb, ss = a.shape, b.shape, sizes.shape
     assert len(sa) == 2 and len(sb) == 3 and len(ss) == 1
     assert sa[1] == sb[1]
@@ -87,6 +97,7 @@ def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:
     assert dev == b.device and dev == sizes.device
     if dtype not in _TYPES:
         raise NotImplementedError(f"gmm supports bf16/fp16/fp32, got {dtype}")
+    refuse_tangents(op, a, b)
     _lib.require_gpu(a)
 
 
@@ -173,7 +184,8 @@ def gmm(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> torch.Tensor:
 def gmm_grad(g: torch.Tensor, a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Gradients (of a, of b) of sum(g * gmm(a, b, sizes)), in the operands' type; zero for rows behind the last group
     and for matrices of empty groups."""
-    _check(a, b, sizes)
+    refuse_tangents("gmm_grad", g)
+    _check(a, b, sizes, "gmm_grad")
     assert g.shape == (a.shape[0], b.shape[2])
     assert g.dtype == a.dtype and g.device == a.device
     T, K = a.shape

@@ -25,7 +25,7 @@ import ctypes
 import torch
 
 from triturus_amd import _lib
-from triturus_amd.gmm import ROW_STRIDE_LIMIT, dense
+from triturus_amd.gmm import ROW_STRIDE_LIMIT, dense, refuse_tangents
 
 BLOCK = 32
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -72,7 +72,7 @@ def _values(x: torch.Tensor) -> torch.Tensor:
 
 
 def mx4_quantize(x: torch.Tensor) -> MX4:
-    """The 4-bit form of x along its last axis."""
+    """The 4-bit form of x along its last axis.  Codes and scales are whole numbers and carry no gradient, as ``torch.argmax``'s."""
     shape = x.shape
     assert len(shape) >= 1
     code = _type_code(x.dtype, "mx4_quantize")
@@ -121,10 +121,13 @@ def mm_mx4(a: torch.Tensor | MX4, b: MX4, sizes: torch.Tensor | None = None, *, 
     """c[r, n] = sum_k a[r, k] b[n, k], or with ``sizes`` b[e(r), n, k]; ``dtype``: of c, by default a's (bf16 for an MX4).
 
     ``_tile`` forces a kernel (tests, timing)."""
+    values = not isinstance(a, MX4)
+    if values:
+        refuse_tangents("mm_mx4", a)
     _check(b)
     bc, bs, K = b
     shape = bc.shape
-    if isinstance(a, MX4):
+    if not values:
         _check(a)
         assert len(a.codes.shape) == 2 and a.length == K
         ac, as_, a_type = _unit(a.codes), _unit(a.scales), -1

@@ -15,7 +15,8 @@ last pair hold row 0, and ``gmm`` gives zeros there.
 Everything stays on the device, in a fixed order: the same logits give the same result bit for bit.
 
 Limits: k <= 16, E <= 1024.  ``weights`` takes part in autograd; under HIP graph capture logits that
-require a gradient are refused, as by ``gmm``: capture ``route`` and ``route_grad`` instead.
+require a gradient are refused, as by ``gmm``: capture ``route`` and ``route_grad`` instead.  ``route_grad`` itself takes no part
+in autograd.  Forward-mode derivatives are refused.
 """
 
 from __future__ import annotations
@@ -26,7 +27,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from triturus_amd import _lib
-from triturus_amd.gmm import refuse_capture
+from triturus_amd.gmm import refuse_capture, refuse_tangents
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _empty = torch.empty_strided
@@ -40,11 +41,12 @@ class Routes(NamedTuple):
     sizes: torch.Tensor    # E, int32: pairs of each expert
 
 
-def _check(logits: torch.Tensor, k: int) -> int:
+def _check(logits: torch.Tensor, k: int, op: str = "route") -> int:
     assert len(logits.shape) == 2
     assert 1 <= k <= logits.shape[1]
     if logits.dtype not in _TYPES:
         raise NotImplementedError(f"route supports bf16/fp16/fp32, got {logits.dtype}")
+    refuse_tangents(op, logits)
     _lib.require_gpu(logits)
     return _lib.DTYPE_CODES[logits.dtype]
 
@@ -124,7 +126,8 @@ def route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Routes:
 
 def route_grad(g: torch.Tensor, logits: torch.Tensor, routes: Routes, *, normalize: bool = True) -> torch.Tensor:
     """Gradient of sum(g * routes.weights) with respect to the logits, in their type; ``normalize`` as in ``route``."""
-    _check(logits, routes.weights.shape[1])
+    refuse_tangents("route_grad", g, routes.weights)
+    _check(logits, routes.weights.shape[1], "route_grad")
     shape = (logits.shape[0], routes.weights.shape[1])
     assert g.shape == routes.weights.shape == routes.experts.shape == shape
     assert g.dtype == routes.weights.dtype == torch.float32 and routes.experts.dtype == torch.int32
