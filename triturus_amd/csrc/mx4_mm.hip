@@ -531,7 +531,7 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
                           int wide_sizes, int tile, void *workspace, size_t workspace_bytes, void *stream) {
     if (!a || (!a_scales && a_type < 0) || !b || !b_scales || !c || !sa || !sb || T <= 0 || E <= 0 || K <= 0 || N <= 0) return TRT_E_INVALID;
     if (!sizes && E != 1) return TRT_E_INVALID;
-    if (a_type > TRT_BF16 || a_type == TRT_F64 || tile < 0 || tile > TRT_MX4_TILES) return TRT_E_INVALID;
+    if (a_type < -1 || a_type > TRT_BF16 || a_type == TRT_F64 || tile < 0 || tile > TRT_MX4_TILES) return TRT_E_INVALID;
     if (dtype != TRT_F32 && dtype != TRT_F16 && dtype != TRT_BF16) return TRT_E_INVALID;
     for (int i = 0; i < 2; ++i)
         if (sa[i] < 0) return TRT_E_LAYOUT;
