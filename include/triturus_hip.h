@@ -357,7 +357,7 @@ size_t trt_gmm_grad_workspace_bytes(const void *g, const void *a, const void *b,
  * codes, row stride of codes, matrix stride of scales, row stride of scales}, all in bytes.  Rows of
  * codes may lie at any address (fastest at multiples of 16 bytes) and at most 8 MiB apart (TRT_E_RANGE).
  * a_type: -1 for codes and scales, or TRT_F32, TRT_F16, TRT_BF16 for T x K values that the call quantises
- * itself (sa[0]: row stride in values; a_scales unused), with a workspace of
+ * itself (sa[0]: row stride in values, as far apart as they like; a_scales unused; K <= 2^24), with a workspace of
  * trt_mx4_mm_workspace_bytes(T, E, K, N, a_type, dtype, tile) bytes, 16-byte aligned; 0 where the product's kernel quantises
  * on the way.  tile: 0 = choose by shape, 1..TRT_MX4_TILES force a tile (experiments, tests).
  */

@@ -537,9 +537,9 @@ extern "C" int trt_mx4_mm(const void *a, const void *a_scales, const void *b, co
         if (sa[i] < 0) return TRT_E_LAYOUT;
     for (int i = 0; i < 4; ++i)
         if (sb[i] < 0) return TRT_E_LAYOUT;
-    // 256 rows of a tile are addressed with 31-bit byte offsets
+    // 256 rows of a tile of codes are addressed with 31-bit byte offsets
     constexpr int64_t kMost = (int64_t)1 << 23;
-    if (sa[0] >= kMost || sb[1] >= kMost || N >= kMost || K > 2 * kMost || T >= (int64_t)1 << 31 || E >= (int64_t)1 << 31) return TRT_E_RANGE;
+    if ((a_type < 0 && sa[0] >= kMost) || sb[1] >= kMost || N >= kMost || K > 2 * kMost || T >= (int64_t)1 << 31 || E >= (int64_t)1 << 31) return TRT_E_RANGE;
     const size_t need = trt_mx4_mm_workspace_bytes(T, E, K, N, a_type, dtype, tile);
     tile = choose_mx4_tile(T, E, K, N, a_type, dtype, tile);
     if (need && (!workspace || workspace_bytes < need)) return TRT_E_WORKSPACE;

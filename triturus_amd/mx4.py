@@ -138,7 +138,7 @@ def mm_mx4(a: torch.Tensor | MX4, b: MX4, sizes: torch.Tensor | None = None, *, 
         a_type = _type_code(a.dtype, "mm_mx4")
         if a.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("mm_mx4 has no gradient: detach its operand")
-        ac = as_ = _values(a) if a.stride(0) < ROW_STRIDE_LIMIT else dense(a)
+        ac = as_ = _values(a)
         dtype = dtype or a.dtype
         sa = _I64x2(ac.stride(0), 0)
     code = _type_code(dtype, "mm_mx4")
