@@ -102,3 +102,38 @@ def test_the_cut_does_not_depend_on_alignment(dev, T, E, K, N, dtype):
     size = torch.stack([a[e * (T // E):(e + 1) * (T // E)].double().abs().T @ g[e * (T // E):(e + 1) * (T // E)].double().abs() for e in range(E)])
     bound = (T // E + 1) * 2.0 ** -23 * size + torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2 ** -8)
     assert ((d.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_pieces_follow_the_rows(dtype):
+    """Few tiles under millions of rows are cut for all CUs, not into as many pieces as under thousands."""
+    for T in (1 << 20, 1 << 22):
+        assert weights(T, 1, 128, 128, dtype) // 65536 >= 192
+        assert weights(T, 2, 128, 256, dtype) // 65536 >= 192
+    assert 2 <= weights(16384, 1, 128, 128, dtype) // 65536 <= 33
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("sizes", [[250000, 49990], [0, 1, 400001], [370003]], ids=str)
+def test_sums_of_many_pieces(dev, sizes, dtype):
+    import torch
+
+    from triturus_amd.gmm import gmm_grad
+
+    K, N, T = 72, 136, sum(sizes) + 10
+    assert weights(T, len(sizes), K, N, dtype) // (2 * 65536) > 95
+    dtype = {code: t for t, code in _lib.DTYPE_CODES.items()}[dtype]
+    a, g, b = torch.randn(T, K, device=dev).to(dtype), (torch.randn(T, N, device=dev) / 64).to(dtype), torch.zeros(len(sizes), K, N, device=dev, dtype=dtype)
+    a[-10:], g[-10:] = math.nan, math.inf
+    s = torch.tensor(sizes, dtype=torch.int32, device=dev)
+    d, r = gmm_grad(g, a, b, s)[1], 0
+    for e, n in enumerate(sizes):
+        x, y = a[r:r + n].double().T, g[r:r + n].double()
+        want, size = x @ y, x.abs() @ y.abs()
+        # every addition within 2^-23 of the running magnitudes, however the rows are cut, and the result's own rounding
+        info = torch.finfo(dtype)
+        bound = (n + 1) * 2.0 ** -23 * size + info.eps / 2 * want.abs() * (1 + 2 ** -8) + info.smallest_normal * info.eps / 2
+        assert ((d[e].double() - want).abs() <= bound).all()
+        r += n
+    assert torch.equal(gmm_grad(g, a, b, s)[1], d)

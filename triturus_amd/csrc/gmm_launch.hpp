@@ -103,6 +103,8 @@ int choose_weights_tile(int64_t E, int64_t K, int64_t N) {
 // That is charged for up to one step of a full CU, two where more than 64 groups are taken as they come: beyond it the tiles come in
 // rounds, over which long and short groups average out (8 groups of 2048 rows, 2056 x 2048 of fp32: 1077 us whole, 1213 in pieces;
 // 9 of 674, 616 x 3000 of bf16: 36 and 72).  The pieces' sums may take 256 MiB, or half of what operands and result take.
+// More than 32 pieces of a group are of 1024 rows or more, and pay for the chain of their sums (479454 rows in 2 groups, 88 x 8 of
+// fp32: 912 us in pieces of 7520 rows, 497 of 1984; 78 shapes of more than 32768 rows a group: 17 -> 10 % behind the best pieces).
 // On 920 random shapes, up to 6000 tiles and 4 million rows, the choice is 6 % behind the best pieces on average and 2.9 times on the
 // worst, whole groups 1.6 and 31 times (16384 rows, 512 x 512 of bf16: 175 us, 29 in pieces; 16 uneven groups, 256 x 512: 48 and 26).
 constexpr double kMostSums = 256 << 20;
@@ -121,12 +123,12 @@ int64_t choose_weights_piece(int64_t T_rows, int64_t E, int64_t K, int64_t N, in
     const double full = E <= kWave ? three : 2 * three;
     double best = 0.97 * (3.3 + steps * larger(mean, longest * (mean < full ? mean : full)));
     int64_t rows = 0;
-    for (int64_t p = 1; p <= 32; ++p) {
+    for (int64_t p = 1; p <= 2048; p += p < 32 ? 1 : p / 8) {
         const int64_t len = ceil_div(ceil_div(T_rows, E * p), 32) * 32;
-        if (len * (int64_t)sizeof(T) < 4 * 64) break;
+        if (len * (int64_t)sizeof(T) < 4 * 64 || (p > 32 && len < 1024)) break;
         if ((double)most_pieces(T_rows, E, len) * matrix * (128 * 128 * sizeof(float)) > larger(kMostSums, 0.5 * held)) break;
         const double n = E == 1 ? (double)ceil_div(T_rows, len) : (double)(T_rows / len) + 0.5 * (double)E, w = n * matrix;
-        const double us = (F32 ? 13.3 : 11.5) + (double)(len * (int64_t)sizeof(T) / 64) * step(w) + w * 0.024;
+        const double us = (F32 ? 13.3 : 11.5) + (double)(len * (int64_t)sizeof(T) / 64) * step(w) + w * 0.024 + (p > 32 ? 0.25 * (double)p : 0.0);
         if (us < best) best = us, rows = len;
     }
     return rows;
