@@ -175,7 +175,7 @@ __device__ __forceinline__ uint32_t divide(uint32_t n, const Divider &v) { retur
 // Groups cut into pieces of len.d rows, the last one of a group shorter, numbered through all groups.  The first lane `want(first,
 // count)` holds for, over all groups' first pieces and their numbers of pieces, says which group it is; rows [start, end) are its own.
 struct GroupPieces {
-    uint32_t group, first, count, start, end;
+    uint32_t first, count, start, end;
 };
 template <typename F>
 __device__ __forceinline__ bool find_pieces(const Sizes &s, const Divider &len, GroupPieces &p, F want) {
@@ -187,7 +187,7 @@ __device__ __forceinline__ bool find_pieces(const Sizes &s, const Divider &len, 
         const uint64_t mask = __ballot(there && want(e + lane_id(), pieces + incl - count, count));
         if (mask) {
             const int who = __builtin_ctzll(mask);
-            p = {e + who, lane_value(pieces + incl - count, who), lane_value(count, who), lane_value(start, who), lane_value(end, who)};
+            p = {lane_value(pieces + incl - count, who), lane_value(count, who), lane_value(start, who), lane_value(end, who)};
             return true;
         }
         pieces += lane_value(incl, kWave - 1);

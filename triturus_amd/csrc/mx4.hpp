@@ -48,7 +48,7 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t codes, const T *v, float 
 }
 
 // 8 codes a word under a block's scale.  The conversion divides by a power of two that has to be a normal number, and takes no
-// subnormal values: blocks below 2^-92 (never fp16's) are moved up by 2^32 before, exactly.
+// subnormal values: blocks whose largest magnitude is below 2^-93 (never fp16's) are moved up by 2^32 before, exactly.
 template <typename T, int N>
 __device__ __forceinline__ void codes_of(const T (&v)[N], uint32_t scale, uint32_t (&codes)[N / 8]) {
 #pragma unroll
