@@ -20,6 +20,8 @@ derivatives are refused.
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
@@ -42,10 +44,12 @@ def refuse_capture(op: str) -> None:
         )
 
 
+# Outside of dual levels (-1) no tensor has a tangent: callers look there first, which costs less than a call.
+dual = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)
+
+
 def refuse_tangents(op: str, *tensors: torch.Tensor) -> None:
     """Operands with a forward-mode tangent: they do not require a gradient, and the result would lose it without a word."""
-    if getattr(forward_ad, "_current_level", 0) < 0:  # outside of dual levels no tensor has one
-        return
     if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{op} has no forward-mode derivative: pass the primal of its operands")
 
@@ -85,7 +89,7 @@ def _few_rows(T: int, E: int) -> bool:
     return T <= 32 * E
 
 
-def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor, op: str = "gmm") -> None:
+def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:
     sa, sb, ss = a.shape, b.shape, sizes.shape
     assert len(sa) == 2 and len(sb) == 3 and len(ss) == 1
     assert sa[1] == sb[1]
@@ -97,7 +101,6 @@ def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor, op: str = "gmm
     assert dev == b.device and dev == sizes.device
     if dtype not in _TYPES:
         raise NotImplementedError(f"gmm supports bf16/fp16/fp32, got {dtype}")
-    refuse_tangents(op, a, b)
     _lib.require_gpu(a)
 
 
@@ -174,6 +177,8 @@ class _Gmm(torch.autograd.Function):
 
 def gmm(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> torch.Tensor:
     """c[r] = a[r] @ b[e(r)], e(r) the group that row r lies in; zeros behind the last group."""
+    if dual._current_level >= 0:
+        refuse_tangents("gmm", a, b)
     _check(a, b, sizes)
     if (a.requires_grad or b.requires_grad) and torch.is_grad_enabled():
         refuse_capture("gmm")
@@ -184,8 +189,9 @@ def gmm(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> torch.Tensor:
 def gmm_grad(g: torch.Tensor, a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Gradients (of a, of b) of sum(g * gmm(a, b, sizes)), in the operands' type; zero for rows behind the last group
     and for matrices of empty groups."""
-    refuse_tangents("gmm_grad", g)
-    _check(a, b, sizes, "gmm_grad")
+    if dual._current_level >= 0:
+        refuse_tangents("gmm_grad", g, a, b)
+    _check(a, b, sizes)
     assert g.shape == (a.shape[0], b.shape[2])
     assert g.dtype == a.dtype and g.device == a.device
     T, K = a.shape

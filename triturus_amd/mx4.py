@@ -25,7 +25,7 @@ import ctypes
 import torch
 
 from triturus_amd import _lib
-from triturus_amd.gmm import ROW_STRIDE_LIMIT, dense, refuse_tangents
+from triturus_amd.gmm import ROW_STRIDE_LIMIT, dense, dual, refuse_tangents
 
 BLOCK = 32
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -121,13 +121,12 @@ def mm_mx4(a: torch.Tensor | MX4, b: MX4, sizes: torch.Tensor | None = None, *, 
     """c[r, n] = sum_k a[r, k] b[n, k], or with ``sizes`` b[e(r), n, k]; ``dtype``: of c, by default a's (bf16 for an MX4).
 
     ``_tile`` forces a kernel (tests, timing)."""
-    values = not isinstance(a, MX4)
-    if values:
+    if dual._current_level >= 0 and not isinstance(a, MX4):
         refuse_tangents("mm_mx4", a)
     _check(b)
     bc, bs, K = b
     shape = bc.shape
-    if not values:
+    if isinstance(a, MX4):
         _check(a)
         assert len(a.codes.shape) == 2 and a.length == K
         ac, as_, a_type = _unit(a.codes), _unit(a.scales), -1

@@ -27,7 +27,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from triturus_amd import _lib
-from triturus_amd.gmm import refuse_capture, refuse_tangents
+from triturus_amd.gmm import dual, refuse_capture, refuse_tangents
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _empty = torch.empty_strided
@@ -41,12 +41,11 @@ class Routes(NamedTuple):
     sizes: torch.Tensor    # E, int32: pairs of each expert
 
 
-def _check(logits: torch.Tensor, k: int, op: str = "route") -> int:
+def _check(logits: torch.Tensor, k: int) -> int:
     assert len(logits.shape) == 2
     assert 1 <= k <= logits.shape[1]
     if logits.dtype not in _TYPES:
         raise NotImplementedError(f"route supports bf16/fp16/fp32, got {logits.dtype}")
-    refuse_tangents(op, logits)
     _lib.require_gpu(logits)
     return _lib.DTYPE_CODES[logits.dtype]
 
@@ -117,6 +116,8 @@ class _Route(torch.autograd.Function):
 
 def route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Routes:
     """The k largest logits of every row, their weights, and the pairs ordered by expert."""
+    if dual._current_level >= 0:
+        refuse_tangents("route", logits)
     if logits.requires_grad and torch.is_grad_enabled():
         _check(logits, k)
         refuse_capture("route")
@@ -126,8 +127,9 @@ def route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Routes:
 
 def route_grad(g: torch.Tensor, logits: torch.Tensor, routes: Routes, *, normalize: bool = True) -> torch.Tensor:
     """Gradient of sum(g * routes.weights) with respect to the logits, in their type; ``normalize`` as in ``route``."""
-    refuse_tangents("route_grad", g, routes.weights)
-    _check(logits, routes.weights.shape[1], "route_grad")
+    if dual._current_level >= 0:
+        refuse_tangents("route_grad", g, logits, routes.weights)
+    _check(logits, routes.weights.shape[1])
     shape = (logits.shape[0], routes.weights.shape[1])
     assert g.shape == routes.weights.shape == routes.experts.shape == shape
     assert g.dtype == routes.weights.dtype == torch.float32 and routes.experts.dtype == torch.int32
