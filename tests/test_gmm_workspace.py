@@ -137,3 +137,12 @@ def test_sums_of_many_pieces(dev, sizes, dtype):
         assert ((d[e].double() - want).abs() <= bound).all()
         r += n
     assert torch.equal(gmm_grad(g, a, b, s)[1], d)
+
+
+def test_aligned_operands_need_the_pieces_alone():
+    """What gmm.py keeps by shape: on the boundaries both queries say the same, wherever the operands lie."""
+    for T, E, K, N, dtype in shapes(5000, 12):
+        K, N = -(-K // 8) * 8, -(-N // 8) * 8
+        w = weights(T, E, K, N, dtype)
+        assert w == grad(T, E, K, N, dtype)
+        assert w == _lib.load().trt_gmm_weights_workspace_bytes(AT + 4096, AT + 16, T, E, K, N, K + 8, N + 64, dtype, 0)

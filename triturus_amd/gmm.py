@@ -89,6 +89,19 @@ def _few_rows(T: int, E: int) -> bool:
     return T <= 32 * E
 
 
+_pieces: dict = {}  # (T, E, K, N, type, tile) -> bytes of the pieces' sums of operands on the boundaries, as reported by the library
+
+
+def _piece_bytes(lib, pa: int, pg: int, T: int, E: int, K: int, N: int, lda: int, ldg: int, code: int, tile: int = 0) -> int:
+    key = (T, E, K, N, code, tile)
+    n = _pieces.get(key)
+    if n is None:
+        if len(_pieces) > 4096:
+            _pieces.clear()
+        n = _pieces[key] = lib.trt_gmm_weights_workspace_bytes(pa, pg, T, E, K, N, lda, ldg, code, tile)
+    return n
+
+
 def _check(a: torch.Tensor, b: torch.Tensor, sizes: torch.Tensor) -> None:
     sa, sb, ss = a.shape, b.shape, sizes.shape
     assert len(sa) == 2 and len(sb) == 3 and len(ss) == 1
@@ -143,11 +156,13 @@ def _weights(a: torch.Tensor, g: torch.Tensor, sizes: torch.Tensor, tile: int = 
     lib, code = _lib.load(), _lib.DTYPE_CODES[dtype]
     pa, pg, lda, ldg = a.data_ptr(), g.data_ptr(), a.stride(0), g.stride(0)
     ws_ptr, nbytes, ws = None, 0, None
-    if (pa | pg) & 15 or (K | N | lda | ldg) & 7 or not _few_rows(T, E):  # a copy or a cut may pay
+    if (pa | pg) & 15 or (K | N | lda | ldg) & 7:  # a copy may pay
         nbytes = lib.trt_gmm_weights_workspace_bytes(pa, pg, T, E, K, N, lda, ldg, code, tile)
-        if nbytes:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            ws_ptr = ws.data_ptr()
+    elif not _few_rows(T, E):
+        nbytes = _piece_bytes(lib, pa, pg, T, E, K, N, lda, ldg, code, tile)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws_ptr = ws.data_ptr()
     with _lib.on_device(dev):
         status = lib.trt_gmm_weights(pa, pg, sizes.data_ptr(), d.data_ptr(), T, E, K, N, lda, ldg, code, sizes.dtype is torch.int64, tile,
                                      ws_ptr, nbytes, _lib.raw_stream(dev))
@@ -205,11 +220,13 @@ def gmm_grad(g: torch.Tensor, a: torch.Tensor, b: torch.Tensor, sizes: torch.Ten
     lib, code = _lib.load(), _lib.DTYPE_CODES[a.dtype]
     pg, pa, pb, ldg, lda, sb = g.data_ptr(), a.data_ptr(), b.data_ptr(), g.stride(0), a.stride(0), _lib.strides3(b)
     ws_ptr, nbytes, ws = None, 0, None
-    if (pg | pa | pb) & 15 or (K | N | ldg | lda | sb[0] | (sb[2] if sb[1] == 1 else sb[1])) & 7 or not _few_rows(T, E):  # a copy or a cut may pay
+    if (pg | pa | pb) & 15 or (K | N | ldg | lda | sb[0] | (sb[2] if sb[1] == 1 else sb[1])) & 7:  # a copy may pay
         nbytes = lib.trt_gmm_grad_workspace_bytes(pg, pa, pb, T, E, K, N, ldg, lda, sb, code)
-        if nbytes:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            ws_ptr = ws.data_ptr()
+    elif not _few_rows(T, E):
+        nbytes = _piece_bytes(lib, pa, pg, T, E, K, N, lda, ldg, code)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws_ptr = ws.data_ptr()
     with _lib.on_device(dev):
         status = lib.trt_gmm_grad(pg, pa, pb, sizes.data_ptr(), da.data_ptr(), db.data_ptr(), T, E, K, N, ldg, lda, sb, code,
                                   sizes.dtype is torch.int64, ws_ptr, nbytes, _lib.raw_stream(dev))
