@@ -375,8 +375,8 @@ size_t trt_mx4_mm_workspace_bytes(int64_t T, int64_t E, int64_t K, int64_t N, in
  * chooses its k largest logits, the lowest index first among equal ones (k <= min(E, 16), E <= 1024, T k < 2^31: TRT_E_RANGE
  * otherwise); -inf is never chosen (such a choice has expert -1, slot -1 and weight 0), a NaN comes first, as in the max
  * reductions.  weights: T x k, the softmax of the chosen logits among themselves (normalize != 0) or among all
- * of the row; a row without a finite choice has zeros.  experts, slots: T x k.  The chosen pairs are ordered by
- * expert, and by row within an expert: slots is a pair's place, rows (T k values) the row at each place (0
+ * of the row; a row of -inf alone has zeros, and a NaN or +inf makes the row's weights NaN.  experts, slots: T x k.  The chosen pairs
+ * are ordered by expert, and by row within an expert: slots is a pair's place, rows (T k values) the row at each place (0
  * behind the last pair), sizes (E values) the experts' numbers of pairs -- the sizes of trt_gmm.  workspace:
  * trt_route_workspace_bytes(T, E) bytes, 16-byte aligned, needing no preparation.  No counterpart in the reference.
  *

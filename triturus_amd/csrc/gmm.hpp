@@ -19,9 +19,10 @@
 // Sums are fp32; a result is rounded once.  The finished tile goes through LDS, so that rows are
 // written 16 bytes a lane.
 //
-// Bound: the matrix pipe and, on 256 x 256 tiles, the card's power: 16384 rows in 8 groups, K = N = 4096 of bf16 take 499 us
-// (1102 TFLOP/s; matrices stored N x K 520 us; the weights' gradient 441 us, 1246) with the pipe busy 69 % of cycles that the
-// clock has stretched to 1.55 GHz.  128 x 128 tiles reach 797 TFLOP/s there (895), fp32 140 (one group of 4096 x 4096 x 4096).
+// Bound: the matrix pipe and, on 256 x 256 tiles, the card's power: 16384 rows in 8 groups, K = N = 4096 of bf16 take 437 to 444 us
+// (1240 TFLOP/s; matrices stored N x K 460 to 470; the weights' gradient 438 to 443; uneven groups 471 to 493), with the pipe busy
+// 69 % of cycles that the clock has stretched to 1.55 GHz.  128 x 128 tiles reach 797 TFLOP/s there (895), fp32 140 (one group of
+// 4096 x 4096 x 4096).
 #pragma once
 
 #include <utility>
@@ -486,7 +487,7 @@ __device__ __forceinline__ void gmm_direct_tile(const T *x, int64_t ldx, const T
         fragments(st0, 0);
         // One way out of the loop: with one behind each step, the compiler joined them before its head, took the loads of any stage
         // to be on their way there, and waited for all of them every fourth step.  (With that, the barrier at the end of a step and
-        // half of the time for the loads, the sizes above took 513 us, and the weights' gradient 454.)
+        // half of the time for the loads, uneven groups of the sizes above took 513 us for 499, and the weights' gradient 454 for 441.)
         int64_t s = 0;
         for (; s + 4 <= steps; s += 4) {
             step(s, st0, st1);

@@ -6,10 +6,11 @@
 // multiplies and scales in one instruction at 4 times the rate of 16-bit operands.  Tiles, staging and LDS
 // layout are those of gmm.hpp (the INNER layout in bytes); the 4 scale bytes of a row's step go with them as
 // one word, from which a lane reads the two of its half: blocks 2 kk + (lane >= 32), kk = 0, 1.  In LDS the words lie [step][row],
-// so that 32 rows' reads lie in different banks (16 bytes apart, as they come from memory, a dense product took 169 us, 158 so).
+// so that 32 rows' reads lie in different banks (16 bytes apart, as they come from memory, a dense product took 169 us for 158).
 //
-// Bound: as for 16-bit operands the card's power, and latency: 8192 x 4096 by 8192 x 4096 to bf16 takes 158 us (3470 TFLOP/s), the
-// matrix pipe busy 46 % of cycles at 1.8 GHz; 16384 rows in 8 groups, K = N = 4096, 192 us (2860).
+// Bound: latency, and a tile's first loads and last stores, beside which a CU has no other tile: 8192 x 4096 by 8192 x 4096 to bf16
+// takes 151 to 158 us (3480 to 3640 TFLOP/s), the matrix pipe busy 46 % of cycles at 1.8 GHz and wavefronts waiting for 32 %; 16384
+// rows in 8 groups, K = N = 4096, 154 to 162 us (uneven groups 169 to 191).
 #include "few.hpp"
 #include "mx4.hpp"
 #include "tile_cost.hpp"

@@ -9,9 +9,9 @@ reference has no counterpart.
     out = (y[r.slots] * r.weights[..., None]).sum(1)        # back to rows, weighted
 
 ``normalize=True``: weights are the softmax of the chosen logits among themselves; ``False``: among all of the row.  Equal logits go
-to the lowest index; a NaN comes first and makes the row's weights NaN.  A logit of -inf is never chosen: its pair has
-expert -1, slot -1, weight 0 and no place in the order, so a row of -inf (padding) takes no expert's time.  Places behind the
-last pair hold row 0, and ``gmm`` gives zeros there.
+to the lowest index; a NaN comes first, and it or +inf makes the row's weights NaN, as in ``torch.softmax``.  A logit of -inf is
+never chosen: its pair has expert -1, slot -1, weight 0 and no place in the order, so a row of -inf (padding) takes no expert's
+time.  Places behind the last pair hold row 0, and ``gmm`` gives zeros there.
 Everything stays on the device, in a fixed order: the same logits give the same result bit for bit.
 
 Limits: k <= 16, E <= 1024.  ``weights`` takes part in autograd; under HIP graph capture logits that
@@ -126,7 +126,8 @@ def route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Routes:
 
 
 def route_grad(g: torch.Tensor, logits: torch.Tensor, routes: Routes, *, normalize: bool = True) -> torch.Tensor:
-    """Gradient of sum(g * routes.weights) with respect to the logits, in their type; ``normalize`` as in ``route``."""
+    """Gradient of sum(g * routes.weights) with respect to the logits, in their type; ``normalize`` and ``routes`` as of ``route``
+    (an expert stands at most once in a row)."""
     if dual._current_level >= 0:
         refuse_tangents("route_grad", g, logits, routes.weights)
     _check(logits, routes.weights.shape[1])
