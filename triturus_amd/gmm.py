@@ -182,6 +182,8 @@ class _Gmm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         refuse_capture("gmm")
+        if dual._current_level >= 0:
+            refuse_tangents("gmm's backward pass", g)
         a, b, sizes = ctx.saved_tensors
         if ctx.needs_input_grad[0] and ctx.needs_input_grad[1]:
             return *gmm_grad(g, a, b, sizes), None

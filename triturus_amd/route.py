@@ -111,6 +111,8 @@ class _Route(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g, *_):
         refuse_capture("route")
+        if dual._current_level >= 0:
+            refuse_tangents("route's backward pass", g)
         return _grad(g, *ctx.saved_tensors, ctx.normalize), None, None
 
 
