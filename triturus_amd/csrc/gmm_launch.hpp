@@ -106,7 +106,7 @@ int choose_weights_tile(int64_t E, int64_t K, int64_t N) {
 // More than 32 pieces of a group are of 1024 rows or more, and pay for the chain of their sums (479454 rows in 2 groups, 88 x 8 of
 // fp32: 912 us in pieces of 7520 rows, 497 of 1984; 78 shapes of more than 32768 rows a group: 17 -> 10 % behind the best pieces).
 // On 920 random shapes, up to 6000 tiles and 4 million rows, the choice is 6 % behind the best pieces on average and 2.9 times on the
-// worst, whole groups 1.6 and 31 times (16384 rows, 512 x 512 of bf16: 175 us, 29 in pieces; 16 uneven groups, 256 x 512: 48 and 26).
+// worst, whole groups 1.6 and 31 times (16384 rows, 512 x 512 of bf16: 175 us, 27 in pieces; 16 uneven groups, 256 x 512: 48 and 26).
 constexpr double kMostSums = 256 << 20;
 template <typename T>
 int64_t choose_weights_piece(int64_t T_rows, int64_t E, int64_t K, int64_t N, int tile) {
